@@ -340,6 +340,103 @@ int qcnn_op_apply_res_float(const void *x, const void *res, void *rec, size_t n,
  * step_w * step_y of both branches agree. */
 int qcnn_concat_steps(float max1, float max2, int step_w1, int step_w2, int *stepy1, int *stepy2);
 
+/* ---- layer level: blocks of language models ------------------------------------------- */
+/* Operators next to the layer-level ones above for networks whose layers are matrix products: a quantised product
+ * with 4-bit weights, products of ragged groups of rows with a weight set each, and the two ends of a residual
+ * block.  No counterpart in the reference.  Arguments come in a structure; a field left 0 / NULL is absent.
+ *   - rows are the first dimension; ld* is the distance between rows in elements (ldw of the 4-bit weights: in
+ *     bytes), at least the row's length; rows, strides and addresses need no alignment beyond the element's own.
+ *   - everything is device memory of the GPU that `stream` belongs to (NULL: the current GPU's default stream).
+ *     The call selects that GPU for its launch and restores the caller's; buffers on another GPU are refused.
+ *   - each call enqueues kernels on `stream`, returns without synchronising, allocates nothing and keeps nothing,
+ *     so calls may overlap on several streams and may be captured into graphs.
+ *   - outputs must not overlap inputs unless the operator says so.
+ *   - results do not depend on the launch: no atomics on values, the same inputs give the same bits.
+ *   - rows == 0 is a call that does nothing.
+ */
+enum {
+    QCNN_F32 = 0,  /* float            */
+    QCNN_F16 = 1,  /* IEEE half        */
+    QCNN_BF16 = 2, /* bfloat16         */
+    QCNN_I8 = 3    /* int8             */
+};
+
+/* Product with 4-bit weights and a scale for each group of `group` inputs:
+ *   y[m][j] = sum_g scale[g][j] * sum_{k in group g} (q[j][k] - zero[g][j]) * x[m][k]  + bias[j]
+ * for any number of rows (made for 1 to 64, where reading the weights is the cost; more rows run in passes of 64).
+ * Sums are float32; the integers q - zero are exact in every path, the result is rounded once.
+ * x must be finite: an infinity may come out as NaN. */
+typedef struct {
+    const void *x;     /* [rows][ldx] of `type`                                                           */
+    void *y;           /* [rows][ldy] of `out_type`                                                       */
+    const void *w;     /* [n][ldw] bytes, two weights a byte: input k = 2i in the low half of byte i      */
+    const void *scale; /* [ceil(k / group)][n] of `scale_type`                                            */
+    const void *zero;  /* uint8 [ceil(k / group)][n], 0..15; NULL: 8 everywhere                           */
+    const void *bias;  /* float [n] or NULL                                                               */
+    size_t ldx, ldy, ldw;
+    int rows, n, k;
+    int group;         /* a multiple of 32; the last group may be short                                   */
+    int type, scale_type, out_type; /* QCNN_F32, QCNN_F16 or QCNN_BF16 each                               */
+} qcnn_matvec_w4_t;
+int qcnn_op_matvec_w4(const qcnn_matvec_w4_t *a, void *stream);
+
+enum { QCNN_ACT_NONE = 0, QCNN_ACT_RELU = 1, QCNN_ACT_SILU = 2 };
+
+/* Products grouped by expert: rows offsets[e] .. offsets[e+1] - 1 of y belong to weight set e,
+ *   y[r][j] = row_scale[r] * act(w_scale[e][j] * x_scale[s] * sum_k w[e][j][k] * x[s][k]  + bias[e][j]),  s = src[r]
+ * The offsets are read on the device; the call's shape depends on `rows` alone, so a captured call may be replayed
+ * with other offsets.  offsets must not decrease; parts of them outside 0 .. rows are cut off.  Rows of y before
+ * offsets[0] and from offsets[experts] on are left as they were.  A row whose src (without src: r itself) is outside
+ * 0 .. x_rows - 1 is taken as a row of zeros.  int8 sums are exact int32 (k <= 131071); the others are float32. */
+typedef struct {
+    const void *x;            /* [x_rows][ldx] of `type`                                                  */
+    void *y;                  /* [rows][ldy] of `out_type`                                                */
+    const void *w;            /* [experts][n][ldw] of `type`, w_stride elements from set to set           */
+    const int32_t *offsets;   /* [experts + 1], device                                                    */
+    const int32_t *src;       /* [rows], device: the row of x that row r of y reads; NULL: r itself       */
+    const float *x_scale;     /* [x_rows] or NULL                                                         */
+    const float *w_scale;     /* [experts][n] or NULL                                                     */
+    const float *bias;        /* [experts][n] or NULL                                                     */
+    const float *row_scale;   /* [rows] or NULL                                                           */
+    size_t ldx, ldy, ldw, w_stride;
+    int rows, x_rows, experts, n, k;  /* experts <= 1024                                                  */
+    int type;                 /* QCNN_F32, QCNN_F16, QCNN_BF16 or QCNN_I8                                 */
+    int out_type;             /* QCNN_F32, QCNN_F16 or QCNN_BF16                                          */
+    int act;                  /* QCNN_ACT_*                                                               */
+} qcnn_grouped_matmul_t;
+int qcnn_op_grouped_matmul(const qcnn_grouped_matmul_t *a, void *stream);
+
+enum { QCNN_NORM_NONE = 0, QCNN_NORM_RMS = 1, QCNN_NORM_LAYER = 2 };
+enum { QCNN_GATE_LINEAR = 0, QCNN_GATE_SIGMOID = 1, QCNN_GATE_TANH = 2, QCNN_GATE_SILU = 3 };
+
+/* The two ends of a residual block in one pass: the norm behind a block, its gate, the scaled residual addition and
+ * the norm before the next block:
+ *   s = sum_{j < parts} y[index[r][j]]        (without index: parts = 1, s = y[r])
+ *   h[r] = beta * x[r] + alpha * act(gate[r / gate_rows]) * post(s)
+ *   n[r] = pre(h[r])                          (of the float32 h, before its rounding)
+ * rms:   v * (w + w_offset) / sqrt(mean(v^2) + eps) + b;  layer: (v - mean(v)) * (w + w_offset) / sqrt(var(v) + eps) + b.
+ * Statistics and sums are float32.  An index outside 0 .. y_rows - 1 adds nothing.  h may be x or (without index) y,
+ * with the same row stride, and n may be either of them that h is not: a row is read before it is written. */
+typedef struct {
+    const void *x;         /* [rows][ldx] of `type`: the residual stream                                  */
+    const void *y;         /* [y_rows][ldy] of `type`: the block's output; NULL: h = beta * x             */
+    const int32_t *index;  /* [rows][parts], device; NULL: row r itself (y_rows >= rows)                  */
+    const void *gate;      /* [ceil(rows / gate_rows)][ldg] of `type`; NULL: 1                            */
+    const void *post_w, *post_b, *pre_w, *pre_b; /* [d] of `w_type`; w NULL: 1, b NULL: 0                 */
+    void *h;               /* [rows][ldh] of `type`; NULL: not written                                    */
+    void *n;               /* [rows][ldn] of `type`; NULL: not written                                    */
+    size_t ldx, ldy, ldg, ldh, ldn;
+    int rows, y_rows, d;   /* d <= 65536                                                                  */
+    int parts;             /* 1 .. 64                                                                     */
+    int gate_rows;         /* rows that share a row of gate, >= 1 where gate is given                     */
+    int type;              /* QCNN_F32, QCNN_F16 or QCNN_BF16                                             */
+    int w_type;            /* QCNN_F32 or `type`                                                          */
+    int post, pre;         /* QCNN_NORM_*                                                                 */
+    int act;               /* QCNN_GATE_*                                                                 */
+    float alpha, beta, post_eps, pre_eps, w_offset;
+} qcnn_norm_res_t;
+int qcnn_op_norm_res(const qcnn_norm_res_t *a, void *stream);
+
 /* ---- device memory helpers for hosts that do not link HIP ------------------------------ */
 int qcnn_set_device(int gpu);
 int qcnn_dev_alloc(void **dev, size_t bytes);

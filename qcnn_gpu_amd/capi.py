@@ -31,6 +31,8 @@ SYMBOLS = (
     "qcnn_load_float", "qcnn_load_float_mem", "qcnn_forward_float", "qcnn_float_w_device_ptr", "qcnn_float_b_device_ptr",
     "qcnn_float_u_device_ptr", "qcnn_op_ppro_float", "qcnn_op_conv_float", "qcnn_op_apply_res_float", "qcnn_hwcn2nchw",
     "qcnn_model_hwcn2nchw",
+    # blocks of language models
+    "qcnn_op_matvec_w4", "qcnn_op_grouped_matmul", "qcnn_op_norm_res",
 )
 
 TAP_X_PPRO, TAP_U_C1, TAP_U_C2_1, TAP_U_C2_2, TAP_U_C3_1, TAP_U_C3_2, TAP_U_C4 = range(7)
@@ -42,6 +44,35 @@ class DynamicState(C.Structure):
     """qcnn_dynamic_state_t of include/qcnn.h."""
     _fields_ = [("stepw", C.c_int32 * 4), ("stepy", C.c_int32 * 4), ("step_w", C.c_int32 * 6),
                 ("step_y", C.c_int32 * 6), ("max_u", C.c_int32 * 6), ("b_adj", C.c_float * 161)]
+
+
+F32, F16, BF16, I8 = range(4)
+ACT_NONE, ACT_RELU, ACT_SILU = range(3)
+NORM_NONE, NORM_RMS, NORM_LAYER = range(3)
+GATE_LINEAR, GATE_SIGMOID, GATE_TANH, GATE_SILU = range(4)
+
+
+def _fields(*groups):
+    return [(name, ctype) for ctype, names in groups for name in names.split()]
+
+
+class MatvecW4(C.Structure):
+    """qcnn_matvec_w4_t of include/qcnn.h."""
+    _fields_ = _fields((C.c_void_p, "x y w scale zero bias"), (C.c_size_t, "ldx ldy ldw"),
+                       (C.c_int, "rows n k group type scale_type out_type"))
+
+
+class GroupedMatmul(C.Structure):
+    """qcnn_grouped_matmul_t of include/qcnn.h."""
+    _fields_ = _fields((C.c_void_p, "x y w offsets src x_scale w_scale bias row_scale"), (C.c_size_t, "ldx ldy ldw w_stride"),
+                       (C.c_int, "rows x_rows experts n k type out_type act"))
+
+
+class NormRes(C.Structure):
+    """qcnn_norm_res_t of include/qcnn.h."""
+    _fields_ = _fields((C.c_void_p, "x y index gate post_w post_b pre_w pre_b h n"), (C.c_size_t, "ldx ldy ldg ldh ldn"),
+                       (C.c_int, "rows y_rows d parts gate_rows type w_type post pre act"),
+                       (C.c_float, "alpha beta post_eps pre_eps w_offset"))
 
 
 class QcnnError(RuntimeError):
@@ -150,6 +181,8 @@ def load():
     L.qcnn_hwcn2nchw.restype = C.c_long
     L.qcnn_hwcn2nchw.argtypes = [vp, i, i, i, i, vp]
     L.qcnn_model_hwcn2nchw.argtypes = [C.c_char_p, C.c_char_p, i]
+    for fn in (L.qcnn_op_matvec_w4, L.qcnn_op_grouped_matmul, L.qcnn_op_norm_res):
+        fn.argtypes = [vp, vp]
     _lib = L
     return L
 

@@ -1,0 +1,66 @@
+// Shared pieces of the operators for blocks of language models (kernels_w4.hip, kernels_grouped.hip, kernels_norm.hip).
+#pragma once
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include "qcnn_internal.h"
+
+namespace qcnn {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+struct bf16_t {
+    uint16_t bits;
+};
+typedef _Float16 f16_t;
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(f16_t v) { return (float)v; }
+__device__ __forceinline__ float to_f32(bf16_t v) { return __uint_as_float((unsigned)v.bits << 16); }
+
+__device__ __forceinline__ void from_f32(float v, float &o) { o = v; }
+__device__ __forceinline__ void from_f32(float v, f16_t &o) { o = (f16_t)v; }
+__device__ __forceinline__ void from_f32(float v, bf16_t &o)  // round to nearest even, v_cvt_pk_bf16_f32
+{
+    const __bf16 r = (__bf16)v;
+    __builtin_memcpy(&o, &r, 2);
+}
+
+// One value of a type known at run time (uniform over the launch): scales, biases and the outputs of the products.
+__device__ __forceinline__ float load_typed(const void *p, size_t i, int type)
+{
+    if (type == QCNN_F32) return ((const float *)p)[i];
+    if (type == QCNN_F16) return (float)((const f16_t *)p)[i];
+    return to_f32(((const bf16_t *)p)[i]);
+}
+__device__ __forceinline__ void store_typed(void *p, size_t i, int type, float v)
+{
+    if (type == QCNN_F32) {
+        ((float *)p)[i] = v;
+    } else if (type == QCNN_F16) {
+        ((f16_t *)p)[i] = (f16_t)v;
+    } else {
+        bf16_t b;
+        from_f32(v, b);
+        ((bf16_t *)p)[i] = b;
+    }
+}
+
+__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + __expf(-v)); }
+
+// ReLU as the library's layers have it, with NaN kept; SiLU v * sigmoid(v), written so that -inf gives -0.
+__device__ __forceinline__ float block_act(float v, int act)
+{
+    if (act == QCNN_ACT_RELU) return v < 0.f ? 0.f : v;
+    if (act == QCNN_ACT_SILU) return v / (1.f + __expf(-v));
+    return v;
+}
+
+hipError_t launch_matvec_w4(const qcnn_matvec_w4_t &a, hipStream_t s);
+hipError_t launch_grouped_matmul(const qcnn_grouped_matmul_t &a, hipStream_t s);
+hipError_t launch_norm_res(const qcnn_norm_res_t &a, hipStream_t s);
+
+}  // namespace qcnn

@@ -9,6 +9,7 @@
 #include <string>
 #include <vector>
 
+#include "block_ops.h"
 #include "qcnn_internal.h"
 
 namespace qcnn {
@@ -1570,6 +1571,152 @@ int qcnn_op_apply_res_float(const void *x, const void *res, void *rec, size_t n,
 {
     if (!x || !res || !rec) return fail(QCNN_E_ARG, "null pointer");
     HIP_TRY(launch_apply_res_float(x, res, rec, n, (hipStream_t)stream));
+    return QCNN_OK;
+}
+
+// ---- blocks of language models -----------------------------------------------------------------
+// What the three entry points share: the GPU of the caller's stream is selected for the launch and the caller's own is
+// restored.  Buffers of another GPU are refused; with one GPU in the machine there is none and nothing is asked.
+namespace {
+class OnStreamDevice {
+  public:
+    explicit OnStreamDevice(hipStream_t s)
+    {
+        err_ = hipGetDevice(&was_);
+        dev_ = was_;
+        if (err_ == hipSuccess && s) err_ = hipStreamGetDevice(s, &dev_);
+        if (err_ == hipSuccess && dev_ != was_) err_ = hipSetDevice(dev_);
+        if (err_ != hipSuccess) (void)hipGetLastError();
+    }
+    ~OnStreamDevice()
+    {
+        if (err_ == hipSuccess && dev_ != was_) (void)hipSetDevice(was_);
+    }
+    hipError_t error() const { return err_; }
+    // true if p may be used on the stream's GPU
+    bool owns(const void *p) const
+    {
+        static const int count = [] {
+            int n = 0;
+            if (hipGetDeviceCount(&n) != hipSuccess) (void)hipGetLastError();
+            return n;
+        }();
+        if (count < 2 || !p) return true;
+        hipPointerAttribute_t at;
+        if (hipPointerGetAttributes(&at, p) != hipSuccess) {
+            (void)hipGetLastError();
+            return true;  // memory the runtime knows nothing of: not ours to judge
+        }
+        return at.type != hipMemoryTypeDevice || at.device == dev_;
+    }
+
+  private:
+    hipError_t err_;
+    int was_ = 0, dev_ = 0;
+};
+
+bool is_float_type(int t) { return t == QCNN_F32 || t == QCNN_F16 || t == QCNN_BF16; }
+size_t type_size(int t) { return t == QCNN_F32 ? 4 : t == QCNN_I8 ? 1 : 2; }
+bool aligned(const void *p, size_t size) { return (uintptr_t)p % size == 0; }
+// The addresses of rows x ld elements have to stay inside 2^63 bytes.
+bool too_far(size_t ld, size_t rows) { return rows && ld > ((size_t)1 << 60) / rows; }
+}  // namespace
+
+#define ON_DEVICE_OF(stream)                                                                                       \
+    OnStreamDevice on((hipStream_t)stream);                                                                        \
+    if (on.error() != hipSuccess) return fail(QCNN_E_HIP, "selecting the stream's GPU failed: %s", hipGetErrorString(on.error()))
+
+int qcnn_op_matvec_w4(const qcnn_matvec_w4_t *a, void *stream)
+{
+    if (!a) return fail(QCNN_E_ARG, "null argument");
+    if (!is_float_type(a->type) || !is_float_type(a->scale_type) || !is_float_type(a->out_type))
+        return fail(QCNN_E_UNSUPPORTED, "types %d, %d, %d: float32, half or bfloat16", a->type, a->scale_type, a->out_type);
+    if (a->rows < 0 || a->n < 1 || a->k < 1) return fail(QCNN_E_ARG, "bad shape: rows %d, n %d, k %d", a->rows, a->n, a->k);
+    if (a->group < 32 || a->group % 32) return fail(QCNN_E_ARG, "group %d: a multiple of 32", a->group);
+    if (a->ldx < (size_t)a->k || a->ldy < (size_t)a->n || a->ldw < ((size_t)a->k + 1) / 2)
+        return fail(QCNN_E_ARG, "row strides %zu, %zu, %zu are shorter than a row", a->ldx, a->ldy, a->ldw);
+    if (too_far(a->ldx, a->rows) || too_far(a->ldy, a->rows) || too_far(a->ldw, a->n)) return fail(QCNN_E_ARG, "row strides too large");
+    if (a->rows == 0) return QCNN_OK;
+    if (!a->x || !a->y || !a->w || !a->scale) return fail(QCNN_E_ARG, "null pointer");
+    if (!aligned(a->x, type_size(a->type)) || !aligned(a->y, type_size(a->out_type)) || !aligned(a->scale, type_size(a->scale_type)) ||
+        !aligned(a->bias, 4))
+        return fail(QCNN_E_ARG, "an address is not aligned to its element");
+    ON_DEVICE_OF(stream);
+    if (!on.owns(a->x) || !on.owns(a->y) || !on.owns(a->w) || !on.owns(a->scale) || !on.owns(a->zero) || !on.owns(a->bias))
+        return fail(QCNN_E_ARG, "a buffer is on another GPU than the stream");
+    HIP_TRY(launch_matvec_w4(*a, (hipStream_t)stream));
+    return QCNN_OK;
+}
+
+int qcnn_op_grouped_matmul(const qcnn_grouped_matmul_t *a, void *stream)
+{
+    if (!a) return fail(QCNN_E_ARG, "null argument");
+    if (!(is_float_type(a->type) || a->type == QCNN_I8) || !is_float_type(a->out_type))
+        return fail(QCNN_E_UNSUPPORTED, "types %d, %d: float32, half, bfloat16 or (inputs) int8", a->type, a->out_type);
+    if (a->act < QCNN_ACT_NONE || a->act > QCNN_ACT_SILU) return fail(QCNN_E_ARG, "unknown activation %d", a->act);
+    if (a->rows < 0 || a->x_rows < 0 || a->n < 1 || a->k < 1)
+        return fail(QCNN_E_ARG, "bad shape: rows %d, x_rows %d, n %d, k %d", a->rows, a->x_rows, a->n, a->k);
+    if (a->experts < 1 || a->experts > 1024) return fail(QCNN_E_UNSUPPORTED, "%d experts (1 to 1024)", a->experts);
+    if (a->type == QCNN_I8 && a->k > 131071) return fail(QCNN_E_UNSUPPORTED, "k %d: int8 sums leave int32 beyond 131071", a->k);
+    if (a->ldx < (size_t)a->k || a->ldy < (size_t)a->n || a->ldw < (size_t)a->k)
+        return fail(QCNN_E_ARG, "row strides %zu, %zu, %zu are shorter than a row", a->ldx, a->ldy, a->ldw);
+    if (too_far(a->ldx, a->x_rows) || too_far(a->ldy, a->rows) || too_far(a->ldw, a->n) || too_far(a->w_stride, a->experts))
+        return fail(QCNN_E_ARG, "strides too large");
+    if (a->rows == 0) return QCNN_OK;
+    if (!a->y || !a->w || !a->offsets || (!a->x && a->x_rows > 0)) return fail(QCNN_E_ARG, "null pointer");
+    if (!aligned(a->x, type_size(a->type)) || !aligned(a->w, type_size(a->type)) || !aligned(a->y, type_size(a->out_type)) ||
+        !aligned(a->offsets, 4) || !aligned(a->src, 4) || !aligned(a->x_scale, 4) || !aligned(a->w_scale, 4) || !aligned(a->bias, 4) ||
+        !aligned(a->row_scale, 4))
+        return fail(QCNN_E_ARG, "an address is not aligned to its element");
+    ON_DEVICE_OF(stream);
+    if (!on.owns(a->x) || !on.owns(a->y) || !on.owns(a->w) || !on.owns(a->offsets) || !on.owns(a->src) || !on.owns(a->x_scale) ||
+        !on.owns(a->w_scale) || !on.owns(a->bias) || !on.owns(a->row_scale))
+        return fail(QCNN_E_ARG, "a buffer is on another GPU than the stream");
+    HIP_TRY(launch_grouped_matmul(*a, (hipStream_t)stream));
+    return QCNN_OK;
+}
+
+int qcnn_op_norm_res(const qcnn_norm_res_t *a, void *stream)
+{
+    if (!a) return fail(QCNN_E_ARG, "null argument");
+    if (!is_float_type(a->type) || !(a->w_type == QCNN_F32 || a->w_type == a->type))
+        return fail(QCNN_E_UNSUPPORTED, "types %d, %d: float32, half or bfloat16, weights float32 or the same", a->type, a->w_type);
+    if (a->post < QCNN_NORM_NONE || a->post > QCNN_NORM_LAYER || a->pre < QCNN_NORM_NONE || a->pre > QCNN_NORM_LAYER)
+        return fail(QCNN_E_ARG, "unknown norm %d / %d", a->post, a->pre);
+    if (a->act < QCNN_GATE_LINEAR || a->act > QCNN_GATE_SILU) return fail(QCNN_E_ARG, "unknown gate %d", a->act);
+    if (a->rows < 0 || a->d < 1) return fail(QCNN_E_ARG, "bad shape: rows %d, d %d", a->rows, a->d);
+    if (a->d > 65536) return fail(QCNN_E_UNSUPPORTED, "d %d: rows of at most 65536", a->d);
+    if (a->post_eps < 0 || a->pre_eps < 0) return fail(QCNN_E_ARG, "negative eps");
+    if (a->rows == 0) return QCNN_OK;
+    const size_t d = a->d;
+    if (!a->x || (!a->h && !a->n)) return fail(QCNN_E_ARG, "null pointer");
+    if (a->index && !a->y) return fail(QCNN_E_ARG, "an index without y");
+    if (a->gate && (!a->y || a->gate_rows < 1)) return fail(QCNN_E_ARG, "a gate needs y and gate_rows >= 1");
+    if (a->y && !a->index && (a->y_rows < a->rows || a->parts > 1))
+        return fail(QCNN_E_ARG, "without index y has a row for each of %d rows (y_rows %d, parts %d)", a->rows, a->y_rows, a->parts);
+    if (a->index && (a->parts < 1 || a->parts > 64 || a->y_rows < 1)) return fail(QCNN_E_ARG, "index: parts %d, y_rows %d", a->parts, a->y_rows);
+    if (a->ldx < d || (a->y && a->ldy < d) || (a->gate && a->ldg < d) || (a->h && a->ldh < d) || (a->n && a->ldn < d))
+        return fail(QCNN_E_ARG, "a row stride is shorter than a row");
+    if (too_far(a->ldx, a->rows) || (a->y && too_far(a->ldy, a->y_rows)) || (a->gate && too_far(a->ldg, a->rows)) ||
+        (a->h && too_far(a->ldh, a->rows)) || (a->n && too_far(a->ldn, a->rows)))
+        return fail(QCNN_E_ARG, "row strides too large");
+    if (a->h && a->h == a->n) return fail(QCNN_E_ARG, "h and n are the same buffer");
+    const size_t t = type_size(a->type), w = type_size(a->w_type);
+    if (!aligned(a->x, t) || !aligned(a->y, t) || !aligned(a->gate, t) || !aligned(a->h, t) || !aligned(a->n, t) || !aligned(a->index, 4) ||
+        !aligned(a->post_w, w) || !aligned(a->post_b, w) || !aligned(a->pre_w, w) || !aligned(a->pre_b, w))
+        return fail(QCNN_E_ARG, "an address is not aligned to its element");
+    if (a->index && (a->h == a->y || a->n == a->y)) return fail(QCNN_E_ARG, "an output over y needs y without index");
+    for (int i = 0; i < 2; ++i) {
+        const void *o = i ? a->n : a->h;
+        const size_t ld = i ? a->ldn : a->ldh;
+        if (o && ((o == a->x && ld != a->ldx) || (o == a->y && ld != a->ldy)))
+            return fail(QCNN_E_ARG, "an output over an input needs its row stride");
+    }
+    ON_DEVICE_OF(stream);
+    if (!on.owns(a->x) || !on.owns(a->y) || !on.owns(a->index) || !on.owns(a->gate) || !on.owns(a->post_w) || !on.owns(a->post_b) ||
+        !on.owns(a->pre_w) || !on.owns(a->pre_b) || !on.owns(a->h) || !on.owns(a->n))
+        return fail(QCNN_E_ARG, "a buffer is on another GPU than the stream");
+    HIP_TRY(launch_norm_res(*a, (hipStream_t)stream));
     return QCNN_OK;
 }
 
