@@ -399,7 +399,7 @@ typedef struct {
     const float *bias;        /* [experts][n] or NULL                                                     */
     const float *row_scale;   /* [rows] or NULL                                                           */
     size_t ldx, ldy, ldw, w_stride;
-    int rows, x_rows, experts, n, k;  /* experts <= 1024                                                  */
+    int rows, x_rows, experts, n, k;  /* experts <= 1024, k <= 2^28                                       */
     int type;                 /* QCNN_F32, QCNN_F16, QCNN_BF16 or QCNN_I8                                 */
     int out_type;             /* QCNN_F32, QCNN_F16 or QCNN_BF16                                          */
     int act;                  /* QCNN_ACT_*                                                               */

@@ -4,6 +4,8 @@
 
 namespace qcnn {
 
+typedef u32x4 u32x4_any __attribute__((aligned(1)));  // global loads and stores take any address
+
 // 16 bytes of a row are a chunk; a matrix instruction of 16 x 16 outputs takes a chunk of every lane: lane l holds
 // chunk (l >> 4) of four of row l & 15.  Both operands come in the same order, so the order of k inside a chunk is free:
 // float32 takes four instructions, element i of every lane's chunk each.
@@ -38,68 +40,160 @@ __device__ __forceinline__ f32x4 mma(float, u32x4 a, u32x4 b, f32x4 c)
     return c;
 }
 
-// The rows of tile `mt` (tiles of TM rows, counted through the experts in turn): expert, first row and row count;
-// false beyond the last tile.  A wave does it alone: 64 experts at a time, their tile counts summed up over the lanes.
-struct RowTile {
-    int e, first, count;
+// A tile of TM rows of one expert and TN outputs.
+struct Tile {
+    int e, first, count, n0;
 };
-__device__ __forceinline__ bool find_tile(const qcnn_grouped_matmul_t &a, int TM, unsigned mt, RowTile &t)
-{
-    const int lane = threadIdx.x & 63;
-    unsigned before = 0;
-    for (int e0 = 0; e0 < a.experts; e0 += 64) {
-        const int e = e0 + lane;
-        int lo = 0, hi = 0;
+
+// The tiles of a call.  They are counted through the experts in turn; workgroups are dealt to the 8 XCDs round robin
+// (blockIdx.x & 7), each with an L2 of its own, so XCD x takes the x-th eighth of the tiles in order, its workgroups one
+// after the other, and inside an expert the order walks bands of 8 row tiles column by column: the 32 workgroups that
+// run on an XCD at a time then share 8 row tiles of x and 4 column tiles of w.
+// The offsets are device memory, so each wave adds up the tiles itself, 64 experts at a time over its lanes.
+template <int TM, int TN>
+struct Tiles {
+    int lo, hi;                // this lane's expert of the first 64, rows [lo, hi)
+    unsigned tiles, sum, all;  // its row tiles, those up to it, those of all experts
+    unsigned nt;               // column tiles
+
+    static __device__ __forceinline__ unsigned scan(const qcnn_grouped_matmul_t &a, int e0, int &lo, int &hi, unsigned &tiles)
+    {
+        const int lane = threadIdx.x & 63, e = e0 + lane;
+        lo = hi = 0;
         if (e < a.experts) {
             lo = min(max(a.offsets[e], 0), a.rows);
             hi = max(min(max(a.offsets[e + 1], 0), a.rows), lo);
         }
-        const unsigned tiles = ((unsigned)(hi - lo) + TM - 1) / TM;
+        tiles = ((unsigned)(hi - lo) + TM - 1) / TM;
         unsigned sum = tiles;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const unsigned u = __shfl_up(sum, o);
             if (lane >= o) sum += u;
         }
-        const unsigned total = __shfl(sum, 63);
-        if (mt < before + total) {
-            const unsigned long long mine = __ballot(mt < before + sum);
-            const int at = __ffsll(mine) - 1;
-            const unsigned start = __shfl(before + sum - tiles, at);
-            lo = __shfl(lo, at);
-            hi = __shfl(hi, at);
-            t.e = __builtin_amdgcn_readfirstlane(e0 + at);
-            t.first = __builtin_amdgcn_readfirstlane(lo + (int)(mt - start) * TM);
-            t.count = __builtin_amdgcn_readfirstlane(min(TM, hi - lo - (int)(mt - start) * TM));
-            return true;
+        return sum;
+    }
+    __device__ __forceinline__ void count(const qcnn_grouped_matmul_t &a)
+    {
+        nt = ((unsigned)a.n + TN - 1) / TN;
+        sum = scan(a, 0, lo, hi, tiles);
+        all = __builtin_amdgcn_readlane(sum, 63);
+        for (int e0 = 64; e0 < a.experts; e0 += 64) {
+            int l, h;
+            unsigned n;
+            all += __builtin_amdgcn_readlane(scan(a, e0, l, h, n), 63);
         }
-        before += total;
     }
-    return false;
-}
-
-// Row tiles a call can have: offsets are device memory, so the grid covers the most that `rows` allows; workgroups
-// without a tile leave.
-static unsigned most_tiles(const qcnn_grouped_matmul_t &a, int TM) { return (unsigned)(a.rows / TM + (a.experts < a.rows ? a.experts : a.rows)); }
-
-// The epilogue of one accumulator (sum) for output j of the expert and row r of y (src row s, `have`: it exists).
-struct Epilogue {
-    float xs, rs;
-    bool have;
-    __device__ __forceinline__ void row(const qcnn_grouped_matmul_t &a, int r, int s, bool exists)
+    // the i-th tile of this workgroup's XCD, false beyond the last
+    __device__ __forceinline__ bool get(const qcnn_grouped_matmul_t &a, unsigned i, Tile &t) const
     {
-        have = exists;
-        xs = a.x_scale && exists ? a.x_scale[s] : 1.f;
-        rs = a.row_scale ? a.row_scale[r] : 1.f;
-    }
-    __device__ __forceinline__ float value(const qcnn_grouped_matmul_t &a, float sum, float ws, float b) const
-    {
-        const float v = have ? sum * ws * xs : 0.f;
-        return block_act(v + b, a.act) * rs;
+        const unsigned per = (all * nt + 7) / 8, at = (blockIdx.x & 7) * per + i;
+        if (i >= per || at >= all * nt) return false;
+        int l0 = lo, h0 = hi, e0 = 0;
+        unsigned n = tiles, s = sum, before = 0;
+        for (;;) {
+            const unsigned total = __builtin_amdgcn_readlane(s, 63);
+            if (at < (before + total) * nt) break;
+            before += total;
+            e0 += 64;  // (at < all * nt: ends inside the experts)
+            s = scan(a, e0, l0, h0, n);
+        }
+        const int l = __ffsll(__ballot(at < (before + s) * nt)) - 1;
+        const unsigned m = __builtin_amdgcn_readlane(n, l), in = at - (before + __builtin_amdgcn_readlane(s, l) - m) * nt;
+        const unsigned band = in / (8 * nt), rows = min(8u, m - band * 8), rest = in - band * 8 * nt;
+        t.e = e0 + l;
+        t.first = __builtin_amdgcn_readlane(l0, l) + (int)(band * 8 + rest % rows) * TM;
+        t.count = min(TM, (int)__builtin_amdgcn_readlane(h0, l) - t.first);
+        t.n0 = (int)(rest / rows) * TN;
+        return true;
     }
 };
 
-typedef u32x4 u32x4_any __attribute__((aligned(1)));
+// Row tiles a call can have: offsets are device memory, so the grid covers the most that `rows` allows (each expert
+// with rows ends in one short tile); workgroups without a tile leave.
+static unsigned most_tiles(const qcnn_grouped_matmul_t &a, int TM) { return (unsigned)(a.rows / TM + (a.experts < a.rows ? a.experts : a.rows)); }
+
+// N neighbouring outputs of one row.  `least` is 0 for ReLU, else -inf (a NaN passes either way).
+template <typename OT, int N>
+__device__ __forceinline__ void store_row(const qcnn_grouped_matmul_t &a, const float (&v)[N], float rs, float least, size_t r, int n)
+{
+    OT o[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) from_f32((v[q] < least ? least : v[q]) * rs, o[q]);
+    OT *y = (OT *)a.y + r * a.ldy + n;
+    if (n + N <= a.n) {
+        constexpr int C = sizeof o / 16;
+        u32x4 c[C];
+        __builtin_memcpy(c, o, sizeof o);
+#pragma unroll
+        for (int i = 0; i < C; ++i) ((u32x4_any *)y)[i] = c[i];
+    } else {
+#pragma unroll
+        for (int q = 0; q < N - 1; ++q)
+            if (n + q < a.n) y[q] = o[q];
+    }
+}
+
+// Outputs of an expert stand in its tiles in another order than in memory: of 32 of them, output 8 g + 4 h + q is row
+// 4 g + q of 16 x 16 tile h.  The lane that holds rows 4 g .. 4 g + 3 of both tiles then has eight neighbouring outputs,
+// 16 bytes of a half row, and four lanes 64 bytes of y (with 8 bytes a lane the stores of a 256 x 256 tile took 20 us, a
+// quarter of the time of 2048 k).
+__device__ __forceinline__ int output_at(int row) { return (row & ~31) | (row >> 2 & 3) << 3 | (row >> 4 & 1) << 2 | (row & 3); }
+
+// The epilogue of a wave's FN x FM accumulators of 16 outputs x 16 rows: the lane has outputs n0 .. n0 + 7 (of each pair
+// of output tiles, 32 further on) of row row0 of each row tile (16 further on); `count` rows of the tile exist.
+template <int FN, int FM, typename A>
+__device__ __forceinline__ void epilogue(const qcnn_grouped_matmul_t &a, const A (&acc)[FN][FM], int e, int first, int row0, int count, int n0)
+{
+    static_assert(FN % 2 == 0, "pairs of output tiles");
+    const float least = a.act == QCNN_ACT_RELU ? 0.f : -__builtin_inff();
+    float xs[FM], rs[FM];
+    bool have[FM];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int row = row0 + i * 16, r = first + min(row, count - 1), s = a.src ? a.src[r] : r;
+        have[i] = s >= 0 && s < a.x_rows;  // of another row what was summed up is dropped
+        xs[i] = a.x_scale && have[i] ? a.x_scale[s] : 1.f;
+        rs[i] = a.row_scale ? a.row_scale[r] : 1.f;
+    }
+    const auto all = [&](auto type) {
+        typedef decltype(type) OT;
+#pragma unroll
+        for (int j = 0; j < FN; j += 2) {
+            const int n = n0 + j * 16;
+            if (n >= a.n) continue;
+            float ws[8], b[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) ws[q] = 1.f, b[q] = 0.f;
+            if (a.w_scale) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) ws[q] = a.w_scale[(size_t)e * a.n + min(n + q, a.n - 1)];
+            }
+            if (a.bias) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) b[q] = a.bias[(size_t)e * a.n + min(n + q, a.n - 1)];
+            }
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                float v[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[q] = (have[i] ? (float)acc[j + (q >> 2)][i][q & 3] * ws[q] * xs[i] : 0.f) + b[q];
+                if (a.act == QCNN_ACT_SILU) {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) v[q] = block_act(v[q], QCNN_ACT_SILU);
+                }
+                if (row0 + i * 16 < count) store_row<OT>(a, v, rs[i], least, (size_t)(first + row0 + i * 16), n);
+            }
+        }
+    };
+    if (a.out_type == QCNN_F32)
+        all(float());
+    else if (a.out_type == QCNN_F16)
+        all(f16_t());
+    else
+        all(bf16_t());
+}
+
 __device__ const u32x4 k_zero_chunk = {0, 0, 0, 0};  // what a lane loads where a row has ended
 
 // Chunk c of a row of `bytes` bytes, at any address; what lies behind the row's end reads as zero.
@@ -128,151 +222,197 @@ __device__ __forceinline__ void load_to_lds(const char *from, unsigned lds)
 }
 
 // ---- tiles through LDS ---------------------------------------------------------------------------------
-// A workgroup of WM x WN waves computes TM rows x TN outputs.  Each step brings 128 bytes of TM rows of x and TN rows of
-// w into one of two LDS buffers while the matrix instructions run on the other; a wave owns TM / WM rows x TN / WN
-// outputs.  Chunk c of tile row i stands in slot c ^ (i >> 1 & 7) of its row: the sixteen lanes that a ds_read_b128
-// serves at a time then touch sixteen different 16-byte slots of the 256 bytes that the banks hold.
+// A workgroup of WM x WN waves computes TM rows x TN outputs, a wave TM / WM x TN / WN of them.  A step is 64 bytes of k:
+// its chunks of TM rows of x and TN rows of w go into one of four LDS buffers, requested four steps before the matrix
+// instructions use them and read into registers one step before: in step s the instructions run on registers, s + 1 is
+// read from LDS, s + 2 and s + 3 are on their way and s + 4 is requested into the buffer that s left.  One barrier a step.
+// Chunk c of tile row i stands in slot c ^ f of the row's four, f = 0, 0, 3, 3 for (i >> 2 & 3): the sixteen lanes that a
+// ds_read_b128 serves at a time (rows 0-3 and 12-15 of one chunk, 4-11 of the next) then touch sixteen different slots
+// of the 256 bytes that the banks hold.
 // ALIGNED (rows begin at multiples of 16 bytes and hold whole chunks): loads go straight to LDS, a lane whose row
-// has ended loads zeros.  Otherwise loads of any address go through registers.
+// has ended loads zeros.  Otherwise loads of any address go through registers, one step ahead.
 template <typename T, int TM, int TN, int WM, int WN, bool ALIGNED>
-__global__ __launch_bounds__(64 * WM *WN, (TM * TN >= 65536 ? 1 : 2)) void k_grouped_tile(const qcnn_grouped_matmul_t a, unsigned nt)
+__global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grouped_matmul_t a)
 {
     constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
     constexpr int FM = TM / WM / 16, FN = TN / WN / 16;             // 16 x 16 tiles of a wave
-    constexpr int LX = TM * 8 / THREADS, LW = TN * 8 / THREADS;     // chunks a thread loads in one step
-    constexpr int BUF = (TM + TN) * 128;
-    static_assert(LX >= 1 && LW >= 1 && TM * 8 % THREADS == 0 && TN * 8 % THREADS == 0, "whole chunks a thread");
+    constexpr int LX = TM * 4 / THREADS, LW = TN * 4 / THREADS;     // chunks a thread loads in one step
+    constexpr int BUF = (TM + TN) * 64;
+    static_assert(LX >= 1 && LW >= 1 && TM * 4 % THREADS == 0 && TN * 4 % THREADS == 0, "whole chunks a thread");
     extern __shared__ __align__(256) char lds[];
     typedef typename Mma<T>::acc_t acc_t;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const unsigned mt = blockIdx.x / nt;
-    const int n0 = (int)(blockIdx.x % nt) * TN;
-    RowTile t;
-    if (!find_tile(a, TM, mt, t)) return;
+    Tiles<TM, TN> tiles;
+    tiles.count(a);
+    Tile t{0, 0, 0, 0}, next_t;
+    unsigned index = blockIdx.x >> 3;
+    if (!tiles.get(a, index, t)) return;
 
-    // this thread's chunks: slot p of tile row i is thread i * 8 + p of a pass; it holds chunk p ^ (i >> 1 & 7)
-    const int bytes = a.k * (int)sizeof(T), slot = tid & 7;
-    const char *xp[LX], *wp[LW];
-    int xc[LX], wc[LW];
+    const int bytes = a.k * (int)sizeof(T);
+    const auto swizzle = [](int row) { return (row >> 3 & 1) * 3; };
+    const char *xp[LX], *wp[LW];  // the rows of which this thread brings a chunk a step
+    static_assert(THREADS % 64 == 0, "all of a thread's chunks stand in the same slot of their rows");
+    const int chunk = ((tid & 3) ^ swizzle(tid >> 2)) * 16;
+    const auto rows_of = [&](const Tile &t) {
 #pragma unroll
-    for (int i = 0; i < LX; ++i) {
-        const int row = (tid + i * THREADS) >> 3;
-        const int r = t.first + min(row, t.count - 1);
-        const int s = a.src ? a.src[r] : r;
-        xp[i] = (const char *)a.x + (size_t)(s >= 0 && s < a.x_rows ? s : 0) * a.ldx * sizeof(T);
-        xc[i] = slot ^ (row >> 1 & 7);
-    }
+        for (int i = 0; i < LX; ++i) {
+            const int r = t.first + min((tid + i * THREADS) >> 2, t.count - 1);
+            const int s = a.src ? a.src[r] : r;
+            xp[i] = (const char *)a.x + (size_t)(s >= 0 && s < a.x_rows ? s : 0) * a.ldx * sizeof(T);
+        }
 #pragma unroll
-    for (int i = 0; i < LW; ++i) {
-        const int row = (tid + i * THREADS) >> 3;
-        wp[i] = (const char *)a.w + ((size_t)t.e * a.w_stride + (size_t)min(n0 + row, a.n - 1) * a.ldw) * sizeof(T);
-        wc[i] = slot ^ (row >> 1 & 7);
-    }
+        for (int i = 0; i < LW; ++i)
+            wp[i] = (const char *)a.w + ((size_t)t.e * a.w_stride + (size_t)min(t.n0 + output_at((tid + i * THREADS) >> 2), a.n - 1) * a.ldw) * sizeof(T);
+    };
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char *)lds;
-    const int steps = (bytes + 127) / 128;
+    const int steps = (bytes + 63) / 64;
     u32x4 held[ALIGNED ? 1 : LX + LW];
-    const auto request = [&](int step, int buf) {
+    const auto request = [&](int step) {
         if constexpr (ALIGNED) {
-            const bool whole = (step + 1) * 128 <= bytes;
-            const unsigned at = lds0 + buf * BUF + wave * 1024;
+            const int from = step * 64 + chunk;
+            const bool ended = from >= bytes;
+            const unsigned at = lds0 + (step & 3) * BUF + wave * 1024;
 #pragma unroll
-            for (int i = 0; i < LX; ++i) {
-                const char *p = xp[i] + (size_t)step * 128 + xc[i] * 16;
-                if (!whole && step * 128 + xc[i] * 16 >= bytes) p = (const char *)&k_zero_chunk;
-                load_to_lds(p, at + i * (THREADS * 16));
-            }
+            for (int i = 0; i < LX; ++i) load_to_lds(ended ? (const char *)&k_zero_chunk : xp[i] + (unsigned)from, at + i * (THREADS * 16));
 #pragma unroll
-            for (int i = 0; i < LW; ++i) {
-                const char *p = wp[i] + (size_t)step * 128 + wc[i] * 16;
-                if (!whole && step * 128 + wc[i] * 16 >= bytes) p = (const char *)&k_zero_chunk;
-                load_to_lds(p, at + TM * 128 + i * (THREADS * 16));
-            }
+            for (int i = 0; i < LW; ++i)
+                load_to_lds(ended ? (const char *)&k_zero_chunk : wp[i] + (unsigned)from, at + TM * 64 + i * (THREADS * 16));
         } else {
 #pragma unroll
-            for (int i = 0; i < LX; ++i) held[i] = load_chunk(xp[i], step * 8 + xc[i], bytes);
+            for (int i = 0; i < LX; ++i) held[i] = load_chunk(xp[i], step * 4 + chunk / 16, bytes);
 #pragma unroll
-            for (int i = 0; i < LW; ++i) held[LX + i] = load_chunk(wp[i], step * 8 + wc[i], bytes);
+            for (int i = 0; i < LW; ++i) held[LX + i] = load_chunk(wp[i], step * 4 + chunk / 16, bytes);
         }
     };
-    const auto deposit = [&](int buf) {
+    const auto deposit = [&](int step) {
         if constexpr (!ALIGNED) {
+            char *at = lds + (step & 3) * BUF + tid * 16;
 #pragma unroll
-            for (int i = 0; i < LX; ++i) *(u32x4 *)(lds + buf * BUF + (tid + i * THREADS) * 16) = held[i];
+            for (int i = 0; i < LX; ++i) *(u32x4 *)(at + i * (THREADS * 16)) = held[i];
 #pragma unroll
-            for (int i = 0; i < LW; ++i) *(u32x4 *)(lds + buf * BUF + TM * 128 + (tid + i * THREADS) * 16) = held[LX + i];
+            for (int i = 0; i < LW; ++i) *(u32x4 *)(at + TM * 64 + i * (THREADS * 16)) = held[LX + i];
         }
     };
 
     const int wm = wave % WM, wn = wave / WM, c16 = lane & 15, g = lane >> 4;
+    const int from = c16 * 64 + (g ^ swizzle(c16)) * 16;  // rows of a wave's tiles begin at multiples of 16
+    struct Frags {
+        u32x4 x[FM], w[FN];
+    };
+    const auto read = [&](int step, Frags &f) {
+        const char *bx = lds + (step & 3) * BUF + wm * (TM / WM) * 64 + from, *bw = lds + (step & 3) * BUF + TM * 64 + wn * (TN / WN) * 64 + from;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) f.x[i] = *(const u32x4 *)(bx + i * 1024);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) f.w[j] = *(const u32x4 *)(bw + j * 1024);
+    };
     acc_t acc[FN][FM];
+    const auto multiply = [&](const Frags &f) {
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
+        for (int j = 0; j < FN; ++j)
 #pragma unroll
-        for (int i = 0; i < FM; ++i) acc[j][i] = acc_t{0, 0, 0, 0};
-
-    request(0, 0);
-    deposit(0);
-    for (int step = 0; step < steps; ++step) {
-        const int buf = step & 1;
-        // this step's chunks have landed, here and (after the barrier) everywhere; everyone is done with the other buffer
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (step + 1 < steps) request(step + 1, buf ^ 1);
-        const char *bx = lds + buf * BUF + (wm * (TM / WM) + c16) * 128, *bw = lds + buf * BUF + TM * 128 + (wn * (TN / WN) + c16) * 128;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int at = ((h * 4 + g) ^ (c16 >> 1)) * 16;  // rows of a wave's tiles begin at multiples of 16
-            u32x4 fx[FM], fw[FN];
-#pragma unroll
-            for (int i = 0; i < FM; ++i) fx[i] = *(const u32x4 *)(bx + i * 2048 + at);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fw[j] = *(const u32x4 *)(bw + j * 2048 + at);
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int i = 0; i < FM; ++i) acc[j][i] = mma(T(), fw[j], fx[i], acc[j][i]);
+            for (int i = 0; i < FM; ++i) acc[j][i] = mma(T(), f.w[j], f.x[i], acc[j][i]);
+    };
+    // The chunks of step s have landed, here and (after the barrier) everywhere, and everyone has read step s - 1 into
+    // registers.  Loads land in order, so all but those of the two steps behind s are waited for.
+    const auto arrive = [&](int s) {
+        if constexpr (ALIGNED) {
+            if (s + 2 < steps)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * (LX + LW)) : "memory");
+            else if (s + 1 < steps)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LX + LW) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        } else {
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
-        if (step + 1 < steps) deposit(buf ^ 1);
-    }
+    };
 
-    // lane: row c16 of each row tile, outputs 4 g .. 4 g + 3 of each output tile
+    Frags f[2];
+    const auto begin = [&] {
+        request(0);
+        if constexpr (ALIGNED) {
+            if (1 < steps) request(1);
+            if (2 < steps) request(2);
+        }
+    };
+    rows_of(t);
+    begin();
+    for (;;) {
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int row = wm * (TM / WM) + i * 16 + c16;
-        if (row >= t.count) continue;
-        const int r = t.first + row, s = a.src ? a.src[r] : r;
-        Epilogue ep;
-        ep.row(a, r, s, s >= 0 && s < a.x_rows);
+        for (int j = 0; j < FN; ++j)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int n = n0 + wn * (TN / WN) + j * 16 + 4 * g;
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (n + q < a.n) {
-                    const size_t o = (size_t)t.e * a.n + n + q;
-                    const float v = ep.value(a, (float)acc[j][i][q], a.w_scale ? a.w_scale[o] : 1.f, a.bias ? a.bias[o] : 0.f);
-                    store_typed(a.y, (size_t)r * a.ldy + n + q, a.out_type, v);
+            for (int i = 0; i < FM; ++i) acc[j][i] = acc_t{0, 0, 0, 0};
+        if constexpr (ALIGNED) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (3 < steps) request(3);
+            read(0, f[0]);
+            const auto step = [&](int s, Frags &now, Frags &next) {
+                if (s + 1 < steps) {
+                    arrive(s + 1);
+                    if (s + 4 < steps) request(s + 4);
+                    read(s + 1, next);
                 }
+                multiply(now);
+            };
+            int s = 0;
+            for (; s + 1 < steps; s += 2) {
+                step(s, f[0], f[1]);
+                step(s + 1, f[1], f[0]);
+            }
+            if (s < steps) step(s, f[0], f[1]);
+        } else {
+            for (int s = 0; s < steps; ++s) {
+                deposit(s);
+                arrive(s);
+                if (s + 1 < steps) request(s + 1);
+                read(s, f[0]);
+                multiply(f[0]);
+            }
         }
+        // the next tile's first chunks are on their way while this one's outputs are written
+        index += gridDim.x >> 3;
+        const bool more = tiles.get(a, index, next_t);
+        if (more) {
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // everyone has read this tile's last chunks
+            rows_of(next_t);
+            begin();
+        }
+        // lane: row c16 of each row tile, outputs 8 g .. 8 g + 7 of each pair of output tiles
+        epilogue(a, acc, t.e, t.first, wm * (TM / WM) + c16, t.count, t.n0 + wn * (TN / WN) + 8 * g);
+        if (!more) break;
+        t = next_t;
     }
+}
+
+// Compute units of the current device, asked for once.
+static int compute_units()
+{
+    static const int n = [] {
+        int dev = 0, cu = 0;
+        if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cu, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cu < 8) cu = 256;
+        return cu;
+    }();
+    return n;
 }
 
 template <typename T, int TM, int TN, int WM, int WN>
 static hipError_t run_tile(const qcnn_grouped_matmul_t &a, bool al, hipStream_t s)
 {
-    const unsigned nt = (unsigned)((a.n + TN - 1) / TN);
-    const unsigned long long blocks = (unsigned long long)most_tiles(a, TM) * nt;
-    if (blocks * (64 * WM * WN) > 0xffffffffull) return hipErrorInvalidConfiguration;
-    constexpr int LDS = 2 * (TM + TN) * 128;
+    constexpr int LDS = 4 * (TM + TN) * 64, PER_CU = 163840 / LDS < 8 / (WM * WN) ? 163840 / LDS : 8 / (WM * WN);
+    const unsigned long long tiles = (unsigned long long)most_tiles(a, TM) * ((a.n + TN - 1) / TN);
+    const unsigned long long fit = (unsigned long long)compute_units() * PER_CU;
+    const unsigned blocks = (unsigned)(((tiles < fit ? tiles : fit) + 7) / 8 * 8);  // as many on each XCD; they walk the tiles
     const void *fn = al ? (const void *)k_grouped_tile<T, TM, TN, WM, WN, true> : (const void *)k_grouped_tile<T, TM, TN, WM, WN, false>;
     if (LDS > 65536) {
         const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) return e;
     }
     if (al)
-        k_grouped_tile<T, TM, TN, WM, WN, true><<<(unsigned)blocks, 64 * WM * WN, LDS, s>>>(a, nt);
+        k_grouped_tile<T, TM, TN, WM, WN, true><<<blocks, 64 * WM * WN, LDS, s>>>(a);
     else
-        k_grouped_tile<T, TM, TN, WM, WN, false><<<(unsigned)blocks, 64 * WM * WN, LDS, s>>>(a, nt);
+        k_grouped_tile<T, TM, TN, WM, WN, false><<<blocks, 64 * WM * WN, LDS, s>>>(a);
     return hipGetLastError();
 }
 
