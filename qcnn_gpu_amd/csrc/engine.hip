@@ -1632,6 +1632,8 @@ int qcnn_op_matvec_w4(const qcnn_matvec_w4_t *a, void *stream)
     if (!is_float_type(a->type) || !is_float_type(a->scale_type) || !is_float_type(a->out_type))
         return fail(QCNN_E_UNSUPPORTED, "types %d, %d, %d: float32, half or bfloat16", a->type, a->scale_type, a->out_type);
     if (a->rows < 0 || a->n < 1 || a->k < 1) return fail(QCNN_E_ARG, "bad shape: rows %d, n %d, k %d", a->rows, a->n, a->k);
+    if (a->n > 1 << 26 || a->ldx > 1u << 24 || a->ldw > 1u << 25)
+        return fail(QCNN_E_UNSUPPORTED, "n %d, row strides %zu and %zu: at most 2^26, 2^24 elements and 2^25 bytes", a->n, a->ldx, a->ldw);
     if (a->group < 32 || a->group % 32) return fail(QCNN_E_ARG, "group %d: a multiple of 32", a->group);
     if (a->ldx < (size_t)a->k || a->ldy < (size_t)a->n || a->ldw < ((size_t)a->k + 1) / 2)
         return fail(QCNN_E_ARG, "row strides %zu, %zu, %zu are shorter than a row", a->ldx, a->ldy, a->ldw);

@@ -6,10 +6,14 @@
 // to 16 rows of x at a time, and the group's scale is applied to the float32 sums of the group, one multiplication for
 // 32 to 128 weights.  One row of x costs as much as sixteen.
 //
-// A workgroup owns 16 NT outputs; its waves split k into runs of whole 128s and their sums meet in LDS at the end.  For
-// 128 k a lane loads 16 bytes of each of its weight rows: lane l, row l & 15, k from (l >> 4) * 32 on.  Instruction j of
-// four wants k = 32 j + (l >> 4) * 8 there, so that its 32 k lie in one group: a 4 x 4 transposition of dwords among the
-// lanes l, l + 16, l + 32, l + 48, four swaps of rows of lanes.
+// The waves of a workgroup are KW x NW: NW share out the outputs, 16 NT each, KW the k, in runs of 128, and the KW sums
+// meet in LDS at the end.  Everything goes through LDS, brought there by direct loads R - 1 runs ahead of its use, so that
+// a wave has kilobytes on their way without registers for them (with loads into registers the compiler's waits left
+// little in flight: 2.8 TB/s).  A wave brings its own codes and scales; x is shared by the NW waves of a k group, one
+// barrier a run, none for NW = 1.
+// Of 128 k a lane holds 16 bytes of each of its weight rows: lane l, row l & 15, k from (l >> 4) * 32 on.  Instruction j
+// of four wants k = 32 j + (l >> 4) * 8 there, so that its 32 k lie in one group: a 4 x 4 transposition of dwords among
+// the lanes l, l + 16, l + 32, l + 48, four swaps of rows of lanes.
 //
 // Codes to half: (w & 0x000f000f) | 0x64006400 is the pair 1024 + q of the nibbles 0 and 4, minus (1024 + z) exact; nibbles
 // 1 and 5 from 0x00f000f0 as 1024 + 16 q, times 1/16 minus (64 + z); the other four the same from w >> 8: 9 operations for
@@ -26,7 +30,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef u32x4 u32x4_any __attribute__((aligned(1)));
 
-constexpr int W4_WAVES = 8;
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 in the clobber lists of the direct loads
 
 // x as it is loaded (RAW registers of 4 for 8 values) and as the matrix instruction takes it (PARTS operands)
 template <typename T>
@@ -132,92 +136,149 @@ __device__ __forceinline__ u32x4 transpose4(u32x4 v)
     return u32x4{c[0], c[1], d[0], d[1]};
 }
 
-// What one wave holds of 128 k: the codes of NT x 16 weight rows, x of MT x 16 rows, the scales (as they stand in memory)
-// and zero points of the groups, one for FL instructions.
-template <typename T, int NT, int MT, int FL>
-struct Stage {
-    u32x4 w[NT], x[MT][4][XForm<T>::RAW];
-    unsigned s[NT][4 / FL];
-    unsigned z[NT][4 / FL];
+// Direct loads to LDS from a uniform address and the lane's offset: lane l's 16 bytes go to lds + 16 l, or its one
+// element of N bytes to lds + 4 l.  (The s_nop holds the wait states that the load
+// needs behind the write of m0, one, and behind a vector instruction's write of the address registers, five.)
+__device__ __forceinline__ void lds_load16(unsigned lds, unsigned offset, const char *base)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void lds_load_one(unsigned lds, unsigned offset, const char *base)
+{
+    if constexpr (N == 1)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_ubyte %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+    else if constexpr (N == 2)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_ushort %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ const char *uniform(const char *p)
+{
+    const unsigned long long u = (unsigned long long)p;
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)u), hi = __builtin_amdgcn_readfirstlane((unsigned)(u >> 32));  // (it returns int)
+    return (const char *)((unsigned long long)hi << 32 | lo);
+}
+
+// LDS of one run of 128 k: x of XROWS rows for the NW waves, then for each wave its codes (1 KB a tile of 16 outputs) and
+// the scales and zero points of its outputs, a dword each, one set for FL instructions.  Chunk c of 16 bytes of x row r stands in slot c ^ (r & 15) of
+// its row: the sixteen lanes that a ds_read_b128 serves at a time read different slots of the 256 bytes that the banks hold.
+template <typename T, int NT, int XROWS, int FL, bool S16, bool ZERO, int KW, int NW, int R>
+struct W4 {
+    static constexpr int WAVES = KW * NW, MT = XROWS < 16 ? 1 : XROWS / 16;
+    static constexpr int XB = XROWS * 128 * (int)sizeof(T), NS = 4 / FL, SB = NS * NT * 64, SI = (SB + 255) / 256;
+    static constexpr int WB = NT * 1024 + SI * 256 * (ZERO ? 2 : 1), RUN = XB + NW * WB;
+    static constexpr int LOADS = NT + XB / 1024 / NW + SI * (ZERO ? 2 : 1);  // direct loads of a wave for one run
+    static constexpr int SUMS = WAVES * NT * MT * 1024;
+    static constexpr int LDS = KW * R * RUN > SUMS ? KW * R * RUN : SUMS;
+    static_assert(XB / 1024 % NW == 0 && NT <= 4 && LOADS * (R - 2) < 64 && LDS <= 163840, "runs fit");
 };
 
-template <typename T, int NT, int MT, int FL, int DEPTH>
-__global__ __launch_bounds__(64 * W4_WAVES) void k_w4(const qcnn_matvec_w4_t a, unsigned nblocks)
+// S16: scales of 16 bits; ZERO: zero points are given.
+template <typename T, int NT, int XROWS, int FL, bool S16, bool ZERO, int KW, int NW, int R>
+__global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, unsigned nblocks)
 {
-    constexpr int PARTS = XForm<T>::PARTS, RAW = XForm<T>::RAW, VE = sizeof(T) == 4 ? 4 : 8;
+    typedef W4<T, NT, XROWS, FL, S16, ZERO, KW, NW, R> G;
+    constexpr int PARTS = XForm<T>::PARTS, RAW = XForm<T>::RAW, MT = G::MT, NS = G::NS, TS = sizeof(T), SS = S16 ? 2 : 4;
     constexpr bool HALF = __is_same(T, f16_t);
-    __shared__ float part[W4_WAVES][NT * 256];
-    __shared__ __align__(16) uint8_t tail_w[16 * 64];
-    __shared__ __align__(16) T tail_x[16 * 128];
-    typedef Stage<T, NT, MT, FL> S;
+    extern __shared__ __align__(1024) char lds[];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
-    const int n0 = (int)(blockIdx.x % nblocks) * 16 * NT, m0 = (int)(blockIdx.x / nblocks) * 16 * MT;
-    const int rows = min(16 * MT, a.rows - m0), row_bytes = (a.k + 1) >> 1;
-    // runs of 256 k (a cache line of a weight row), as equal as they can be
-    const int units = (a.k + 255) >> 8, blocks = (a.k + 127) >> 7;
-    const int kb0 = min(blocks, 2 * (int)((long long)units * wave / W4_WAVES)), kb1 = min(blocks, 2 * (int)((long long)units * (wave + 1) / W4_WAVES));
+    const int kq = wave / NW, nq = wave % NW;
+    const int n0 = ((int)(blockIdx.x % nblocks) * NW + nq) * 16 * NT, m0 = (int)(blockIdx.x / nblocks) * XROWS;
+    const int rows = min(XROWS, a.rows - m0), row_bytes = (a.k + 1) >> 1;
 
-    const uint8_t *wrow[NT];
-    int col[NT];
+    // runs of this k group: pairs, as two runs share the cache lines of the weight rows; the last run of all may be cut by
+    // the end of the rows.  Every wave of the workgroup makes `turns` turns.
+    const int all = (a.k + 127) >> 7, turns = ((all + 1) / 2 + KW - 1) / KW * 2;
+    const int first = kq * turns, count = max(0, min(turns, all - first));
+    const bool cut = a.k % 128 != 0 && first + count == all && count > 0;
+    const int whole = count - (cut ? 1 : 0);
+
+    // this lane's sources, as offsets from uniform addresses (ldw and ldx are at most 2^25 and 2^24)
+    unsigned wat[NT], xat[G::XB / 1024 / NW];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        col[t] = min(n0 + t * 16 + c16, a.n - 1);
-        wrow[t] = (const uint8_t *)a.w + (size_t)col[t] * a.ldw;
+    for (int t = 0; t < NT; ++t) wat[t] = (unsigned)max(0, min(t * 16 + c16, a.n - 1 - n0)) * (unsigned)a.ldw + g * 16;
+    constexpr int CPR = 8 * TS;  // chunks of an x row
+#pragma unroll
+    for (int i = 0; i < G::XB / 1024 / NW; ++i) {
+        const int at = (i * NW + nq) * 64 + lane, row = at / CPR;
+        xat[i] = (unsigned)min(row, rows - 1) * (unsigned)(a.ldx * TS) + ((at % CPR) ^ (row & 15)) * 16;
     }
-    const T *xrow[MT];
+    // scale e = 64 i + lane of a run: of set e / 16 NT, output e % 16 NT
+    unsigned col[G::SI];
+    int set[G::SI];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) xrow[m] = (const T *)a.x + (size_t)(m0 + min(m * 16 + c16, rows - 1)) * a.ldx;
-    const unsigned per = (unsigned)a.group >> 5;
+    for (int i = 0; i < G::SI; ++i) {
+        set[i] = min((i * 64 + lane) / (16 * NT), NS - 1);
+        col[i] = (unsigned)max(0, min((i * 64 + lane) % (16 * NT), a.n - 1 - n0));
+    }
+    const int nbase = min(n0, a.n - 1);  // (a wave beyond the outputs reads the last one's and stores nothing)
+    const char *const w0 = (const char *)a.w + (size_t)nbase * a.ldw, *const x0 = (const char *)a.x + (size_t)m0 * a.ldx * TS;
+    const unsigned per = (unsigned)a.group >> 5, last = (unsigned)(a.k - 1) / (unsigned)a.group;
+    char *const ring = lds + kq * (R * G::RUN);
+    const unsigned ring_at = (unsigned)(size_t)(__attribute__((address_space(3))) char *)ring;
 
-    const auto load_scales = [&](S &st, int kb) {
+    unsigned gi = (unsigned)first * 4 / per, left = per - (unsigned)first * 4 % per;  // group of the next run to bring, its 32s of k left
+    const auto next_scales = [&](size_t &from, unsigned (&offset)[G::SI]) {  // elements: of the first set, and of each lane's from there
+        unsigned group[NS];
 #pragma unroll
-        for (int f = 0; f < 4 / FL; ++f) {
-            const int k32 = min(kb * 4 + f * FL, (a.k - 1) >> 5);  // (behind the last group: x is zero there)
-            const size_t at = (size_t)((unsigned)k32 / per) * a.n;
+        for (int f = 0; f < NS; ++f) {
+            group[f] = min(gi, last);  // (behind the last group x is zero)
+            left -= FL;
+            if (left == 0) ++gi, left = per;
+        }
+        from = (size_t)group[0] * a.n + nbase;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                st.s[t][f] = a.scale_type == QCNN_F32 ? ((const unsigned *)a.scale)[at + col[t]] : ((const uint16_t *)a.scale)[at + col[t]];
-                st.z[t][f] = a.zero ? ((const uint8_t *)a.zero)[at + col[t]] : 8;
+        for (int i = 0; i < G::SI; ++i) {
+            offset[i] = col[i];
+#pragma unroll
+            for (int f = 1; f < NS; ++f)
+                if (set[i] == f) offset[i] += (group[f] - group[0]) * (unsigned)a.n;  // (n <= 2^26)
+        }
+    };
+    // brings run i (of this group) into the ring
+    const auto bring = [&](int i) {
+        const int kb = first + i, slot = i % R;
+        if (i < whole) {
+            const unsigned at = ring_at + slot * G::RUN, mine = at + G::XB + nq * G::WB;
+            const char *w = uniform(w0 + (size_t)kb * 64), *x = uniform(x0 + (size_t)kb * (128 * TS));
+#pragma unroll
+            for (int t = 0; t < NT; ++t) lds_load16(mine + t * 1024, wat[t], w);
+#pragma unroll
+            for (int j = 0; j < G::XB / 1024 / NW; ++j) lds_load16(at + (j * NW + nq) * 1024, xat[j], x);
+            size_t from;
+            unsigned offset[G::SI];
+            next_scales(from, offset);
+#pragma unroll
+            for (int j = 0; j < G::SI; ++j) {
+                lds_load_one<SS>(mine + NT * 1024 + j * 256, offset[j] * SS, uniform((const char *)a.scale + from * SS));
+                if (ZERO) lds_load_one<1>(mine + NT * 1024 + (G::SI + j) * 256, offset[j], uniform((const char *)a.zero + from));
             }
-        }
-    };
-    const auto load = [&](S &st, int kb) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) st.w[t] = *(const u32x4_any *)(wrow[t] + (size_t)kb * 64 + g * 16);
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int r = 0; r < RAW; ++r) {
-                    // of sixteen rows only those that there are ask for x; the others' sums are not stored
-                    if (MT > 1 || c16 < rows) st.x[m][j][r] = *(const u32x4_any *)(xrow[m] + kb * 128 + j * 32 + g * 8 + r * 4);
-                }
-        load_scales(st, kb);
-    };
-    // The last 128 k where the rows end inside them: x and the codes come through LDS, zeros behind the end of x
-    const auto load_tail = [&](S &st, int kb) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            for (int i = g; i < 64; i += 4) tail_w[c16 * 64 + i] = kb * 64 + i < row_bytes ? wrow[t][(size_t)kb * 64 + i] : 0;
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            st.w[t] = *(const u32x4 *)(tail_w + c16 * 64 + g * 16);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
+        } else if (cut && i == whole) {  // element by element, zeros behind the end of x
+            char *at = ring + slot * G::RUN, *mine = at + G::XB + nq * G::WB;
+            for (int e = lane; e < NT * 1024; e += 64) {  // byte e & 63 of weight row e >> 6; lane (row & 15) + 16 (byte >> 4) reads it
+                const int row = e >> 6, byte = e & 63;
+                mine[(row >> 4) * 1024 + ((byte >> 4) * 16 + (row & 15)) * 16 + (byte & 15)] =
+                    kb * 64 + byte < row_bytes && n0 + row < a.n ? w0[(size_t)row * a.ldw + kb * 64 + byte] : 0;
+            }
             T zero;
             from_f32(0.f, zero);
-            for (int i = g; i < 128; i += 4) tail_x[c16 * 128 + i] = kb * 128 + i < a.k ? xrow[m][kb * 128 + i] : zero;
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            for (int e = nq * 64 + lane; e < XROWS * 128; e += NW * 64) {
+                const int row = e >> 7, k = e & 127, c = k * TS / 16;
+                *(T *)(at + row * (128 * TS) + (c ^ (row & 15)) * 16 + k * TS % 16) =
+                    kb * 128 + k < a.k ? ((const T *)x0)[(size_t)min(row, rows - 1) * a.ldx + kb * 128 + k] : zero;
+            }
+            size_t from;
+            unsigned offset[G::SI];
+            next_scales(from, offset);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int r = 0; r < RAW; ++r) st.x[m][j][r] = *(const u32x4 *)(tail_x + c16 * 128 + j * 32 + g * 8 + r * 4);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            for (int j = 0; j < G::SI; ++j) {
+                unsigned *sz = (unsigned *)(mine + NT * 1024 + j * 256) + lane;
+                *sz = S16 ? ((const uint16_t *)a.scale)[from + offset[j]] : ((const unsigned *)a.scale)[from + offset[j]];
+                if (ZERO) sz[G::SI * 64] = ((const uint8_t *)a.zero)[from + offset[j]];
+            }
         }
-        load_scales(st, kb);
     };
 
     f32x4 acc[NT][MT];
@@ -225,31 +286,48 @@ __global__ __launch_bounds__(64 * W4_WAVES) void k_w4(const qcnn_matvec_w4_t a, 
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[t][m] = f32x4{0, 0, 0, 0};
+    const bool bf16_scales = a.scale_type == QCNN_BF16;
 
-    const auto compute = [&](const S &st) {
+    const auto consume = [&](int i) {
+        const char *at = ring + i % R * G::RUN, *mine = at + G::XB + nq * G::WB;
         u32x4 w[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) w[t] = transpose4(st.w[t]);
-        f32x4 sum[NT][MT], ones[MT];
+        for (int t = 0; t < NT; ++t) w[t] = transpose4(*(const u32x4 *)(mine + t * 1024 + lane * 16));
 #pragma unroll
-        for (int f = 0; f < 4 / FL; ++f) {
-            if (f) __builtin_amdgcn_sched_barrier(0);  // one group's registers at a time
+        for (int f = 0; f < NS; ++f) {
+            f32x4 sum[NT][MT], ones[MT];
+            float s[NT], z[NT];
+            HalfZero hz[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const char *p = mine + NT * 1024 + (f * 16 * NT + t * 16 + c16) * 4;
+                if (S16) {
+                    const unsigned u = *(const uint16_t *)p;
+                    s[t] = bf16_scales ? __uint_as_float(u << 16) : (float)__builtin_bit_cast(f16_t, (uint16_t)u);
+                } else {
+                    s[t] = *(const float *)p;
+                }
+                z[t] = ZERO ? (float)*(const uint8_t *)(p + G::SI * 256) : 8.f;
+                hz[t] = half_zero(z[t]);
+            }
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 ones[m] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int t = 0; t < NT; ++t) sum[t][m] = f32x4{0, 0, 0, 0};
             }
-            HalfZero hz[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) hz[t] = half_zero((float)st.z[t][f]);
 #pragma unroll
             for (int j = f * FL; j < (f + 1) * FL; ++j) {
                 u32x4 x[MT][PARTS];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    x_operand(T(), st.x[m][j], x[m]);
-                    if (!HALF && a.zero) {
+                    const int row = XROWS < 16 ? c16 % XROWS : m * 16 + c16;
+                    u32x4 raw[RAW];
+#pragma unroll
+                    for (int r = 0; r < RAW; ++r)
+                        raw[r] = *(const u32x4 *)(at + row * (128 * TS) + (((j * 4 + g) * RAW + r) ^ (row & 15)) * 16);
+                    x_operand(T(), raw, x[m]);
+                    if (!HALF && ZERO) {
                         const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
                         for (int p = 0; p < PARTS; ++p) ones[m] = mma(T(), x[m][p], one, ones[m]);
@@ -259,94 +337,96 @@ __global__ __launch_bounds__(64 * W4_WAVES) void k_w4(const qcnn_matvec_w4_t a, 
                 for (int t = 0; t < NT; ++t) {
                     const u32x4 c = codes(T(), w[t][j], hz[t]);
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) {
+                    for (int m = 0; m < MT; ++m)
 #pragma unroll
                         for (int p = 0; p < PARTS; ++p) sum[t][m] = mma(T(), x[m][p], c, sum[t][m]);
-                    }
                 }
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const unsigned u = st.s[t][f];
-                float s = __uint_as_float(a.scale_type == QCNN_BF16 ? u << 16 : u);
-                if (a.scale_type == QCNN_F16) s = (float)__builtin_bit_cast(f16_t, (uint16_t)u);
-                const float s16 = HALF ? s : 16.f * s, sz = s * (8.f - (float)st.z[t][f]);
+                const float s16 = HALF ? s[t] : 16.f * s[t], sz = s[t] * (8.f - z[t]);
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        acc[t][m][i] = fmaf(s16, sum[t][m][i], acc[t][m][i]);
-                        if (!HALF && a.zero) acc[t][m][i] = fmaf(sz, ones[m][i], acc[t][m][i]);
+                    for (int q = 0; q < 4; ++q) {
+                        acc[t][m][q] = fmaf(s16, sum[t][m][q], acc[t][m][q]);
+                        if (!HALF && ZERO) acc[t][m][q] = fmaf(sz, ones[m][q], acc[t][m][q]);
                     }
             }
         }
     };
 
-    const bool cut = a.k % 128 != 0 && kb1 == blocks && kb0 < kb1;  // this wave has the end of the rows
-    const int whole = kb1 - (cut ? 1 : 0);
-    S st[DEPTH];
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-        if (MT == 1) {  // lanes without a row keep zeros
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int r = 0; r < RAW; ++r) st[d].x[0][j][r] = u32x4{0, 0, 0, 0};
-        }
-        if (kb0 + d < whole) load(st[d], kb0 + d);
-    }
-    for (int kb = kb0; kb < whole; kb += DEPTH) {
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
-            if (kb + d >= whole) break;
-            compute(st[d]);
-            if (kb + d + DEPTH < whole) load(st[d], kb + d + DEPTH);
-        }
-    }
-    if (cut) {
-        load_tail(st[0], whole);
-        compute(st[0]);
+    for (int i = 0; i < R - 1; ++i) bring(i);
+    for (int i = 0; i < turns; ++i) {
+        // run i has landed (loads land in order: all but those of the runs behind it), here and after the barrier for all,
+        // and everyone is done with run i - 1, whose place run i + R - 1 takes
+        const int behind = min(R - 2, whole - 1 - i);
+        if (R > 3 && behind >= 2)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(G::LOADS * 2) : "memory");
+        else if (R > 2 && behind >= 1)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(G::LOADS) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (NW > 1) asm volatile("s_barrier" ::: "memory");
+        bring(i + R - 1);
+        if (i < count) consume(i);
     }
 
-    // the waves' sums, 16 rows at a time; the lane has rows 4 g .. 4 g + 3 of output c16 of each tile
+    // the k groups' sums; the lane has rows 4 g .. 4 g + 3 of output c16 of each tile
+    __syncthreads();
+    float *sums = (float *)lds;
+    constexpr int OUT = 16 * NT * NW;  // outputs of the workgroup
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        if (m * 16 >= rows) break;
-        if (m) __syncthreads();
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[wave][(4 * g + i) * (16 * NT) + t * 16 + c16] = acc[t][m][i];
-        __syncthreads();
-        for (int o = threadIdx.x; o < NT * 256; o += 64 * W4_WAVES) {
-            const int row = m * 16 + o / (16 * NT), j = n0 + o % (16 * NT);
-            if (row >= rows || j >= a.n) continue;
-            float v = 0.f;
+            for (int q = 0; q < 4; ++q) sums[kq * (OUT * 16 * MT) + (m * 16 + 4 * g + q) * OUT + nq * (16 * NT) + t * 16 + c16] = acc[t][m][q];
+    __syncthreads();
+    const int base = (int)(blockIdx.x % nblocks) * OUT;
+    for (int o = threadIdx.x; o < OUT * rows; o += 64 * KW * NW) {
+        const int row = o / OUT, j = base + o % OUT;
+        if (j >= a.n) continue;
+        float v = 0.f;
 #pragma unroll
-            for (int w = 0; w < W4_WAVES; ++w) v += part[w][o];
-            if (a.bias) v += ((const float *)a.bias)[j];
-            store_typed(a.y, (size_t)(m0 + row) * a.ldy + j, a.out_type, v);
-        }
+        for (int k = 0; k < KW; ++k) v += sums[k * (OUT * 16 * MT) + o];
+        if (a.bias) v += ((const float *)a.bias)[j];
+        store_typed(a.y, (size_t)(m0 + row) * a.ldy + j, a.out_type, v);
     }
 }
 
-template <typename T, int NT, int MT, int FL, int DEPTH>
+template <typename T, int NT, int XROWS, int FL, bool S16, bool ZERO, int KW, int NW, int R>
+static hipError_t launch(const qcnn_matvec_w4_t &a, hipStream_t s)
+{
+    typedef W4<T, NT, XROWS, FL, S16, ZERO, KW, NW, R> G;
+    const unsigned nblocks = (unsigned)((a.n + 16 * NT * NW - 1) / (16 * NT * NW));
+    const unsigned long long blocks = (unsigned long long)nblocks * ((a.rows + XROWS - 1) / XROWS);
+    if (blocks * (64 * G::WAVES) > 0xffffffffull) return hipErrorInvalidConfiguration;
+    const auto fn = k_w4<T, NT, XROWS, FL, S16, ZERO, KW, NW, R>;
+    if (G::LDS > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
+        if (e != hipSuccess) return e;
+    }
+    fn<<<(unsigned)blocks, 64 * G::WAVES, G::LDS, s>>>(a, nblocks);
+    return hipGetLastError();
+}
+
+template <typename T, int NT, int XROWS, int FL, int KW, int NW, int R>
 static hipError_t run(const qcnn_matvec_w4_t &a, hipStream_t s)
 {
-    const unsigned nblocks = (unsigned)((a.n + 16 * NT - 1) / (16 * NT));
-    const unsigned long long blocks = (unsigned long long)nblocks * ((a.rows + 16 * MT - 1) / (16 * MT));
-    if (blocks * (64 * W4_WAVES) > 0xffffffffull) return hipErrorInvalidConfiguration;
-    k_w4<T, NT, MT, FL, DEPTH><<<(unsigned)blocks, 64 * W4_WAVES, 0, s>>>(a, nblocks);
-    return hipGetLastError();
+    if (a.scale_type != QCNN_F32)
+        return a.zero ? launch<T, NT, XROWS, FL, true, true, KW, NW, R>(a, s) : launch<T, NT, XROWS, FL, true, false, KW, NW, R>(a, s);
+    return a.zero ? launch<T, NT, XROWS, FL, false, true, KW, NW, R>(a, s) : launch<T, NT, XROWS, FL, false, false, KW, NW, R>(a, s);
 }
 
 template <typename T, int FL>
 static hipError_t pick_rows(const qcnn_matvec_w4_t &a, hipStream_t s)
 {
-    if (a.rows > 32) return run<T, 2, 4, FL, 1>(a, s);
-    if (a.rows > 16) return run<T, 4, 2, FL, 1>(a, s);
-    if (a.rows > 4 && a.n > 4096) return run<T, 4, 1, FL, 2>(a, s);
-    return run<T, 1, 1, FL, 3>(a, s);
+    constexpr bool F = sizeof(T) == 4;
+    if (a.rows > 16) return run<T, 1, F ? 32 : 64, FL, 2, 4, 3>(a, s);
+    if (a.rows > 4) return run<T, 1, 16, FL, 2, 4, F ? 3 : 4>(a, s);
+    return run<T, 1, 4, FL, 8, 1, FL == 1 ? 3 : 4>(a, s);
 }
 
 template <typename T>

@@ -29,8 +29,8 @@ def norm(**kw):
 
 REFUSED = [
     (w4, dict(type=3), E_UNSUPPORTED), (w4, dict(scale_type=9), E_UNSUPPORTED), (w4, dict(out_type=-1), E_UNSUPPORTED),
-    (w4, dict(rows=-1), E_ARG), (w4, dict(n=0), E_ARG), (w4, dict(k=0), E_ARG), (w4, dict(group=0), E_ARG), (w4, dict(group=48), E_ARG),
-    (w4, dict(group=-32), E_ARG), (w4, dict(ldx=63), E_ARG), (w4, dict(ldy=7), E_ARG), (w4, dict(ldw=31), E_ARG), (w4, dict(ldw=1 << 62), E_ARG),
+    (w4, dict(rows=-1), E_ARG), (w4, dict(n=0), E_ARG), (w4, dict(k=0), E_ARG), (w4, dict(n=(1 << 26) + 1, ldy=1 << 29), E_UNSUPPORTED), (w4, dict(ldx=(1 << 24) + 1), E_UNSUPPORTED), (w4, dict(ldw=(1 << 25) + 1), E_UNSUPPORTED), (w4, dict(group=0), E_ARG), (w4, dict(group=48), E_ARG),
+    (w4, dict(group=-32), E_ARG), (w4, dict(ldx=63), E_ARG), (w4, dict(ldy=7), E_ARG), (w4, dict(ldw=31), E_ARG), (w4, dict(ldw=1 << 62), E_UNSUPPORTED),
     (w4, dict(k=63, ldx=63, ldw=31), E_ARG), (w4, dict(x=None), E_ARG), (w4, dict(y=None), E_ARG), (w4, dict(w=None), E_ARG), (w4, dict(scale=None), E_ARG),
     (w4, dict(x=A + 1), E_ARG), (w4, dict(scale=A + 1), E_ARG), (w4, dict(bias=A + 2), E_ARG), (w4, dict(y=A + 2, out_type=capi.F32), E_ARG),
     (grouped, dict(type=4), E_UNSUPPORTED), (grouped, dict(out_type=capi.I8), E_UNSUPPORTED), (grouped, dict(act=3), E_ARG), (grouped, dict(act=-1), E_ARG),
