@@ -2,31 +2,31 @@
 //   y[m][j] = sum_g s[g][j] sum_{k in g} (q[j][k] - z[g][j]) x[m][k] + b[j]
 //
 // Reading the weights is the cost, n * k / 2 bytes; everything else has to keep out of their way.  The codes become
-// exact small integers in the type of the matrix instruction (half or bfloat16), 16 x 16 x 32 tiles multiply them with up
+// exact small numbers in the type of the matrix instruction (half or bfloat16), 16 x 16 x 32 tiles multiply them with up
 // to 16 rows of x at a time, and the group's scale is applied to the float32 sums of the group, one multiplication for
 // 32 to 128 weights.  One row of x costs as much as sixteen.
 //
 // The waves of a workgroup are KW x NW: NW share out the outputs, 16 NT each, KW the k, in runs of 128, and the KW sums
 // meet in LDS at the end.  Everything goes through LDS, brought there by direct loads R - 1 runs ahead of its use, so that
-// a wave has kilobytes on their way without registers for them (with loads into registers the compiler's waits left
-// little in flight: 2.8 TB/s).  A wave brings its own codes and scales; x is shared by the NW waves of a k group, one
+// a wave has kilobytes on their way without registers for them.  A wave issues an instruction every seven cycles or so, so
+// instructions a run and waves on a CU set the pace where the memory does not.  A wave brings its own codes and scales; x is shared by the NW waves of a k group, one
 // barrier a run, none for NW = 1.
 // Of 128 k a lane holds 16 bytes of each of its weight rows: lane l, row l & 15, k from (l >> 4) * 32 on.  Instruction j
 // of four wants k = 32 j + (l >> 4) * 8 there, so that its 32 k lie in one group: a 4 x 4 transposition of dwords among
 // the lanes l, l + 16, l + 32, l + 48, four swaps of rows of lanes.
 //
-// Codes to half: (w & 0x000f000f) | 0x64006400 is the pair 1024 + q of the nibbles 0 and 4, minus (1024 + z) exact; nibbles
-// 1 and 5 from 0x00f000f0 as 1024 + 16 q, times 1/16 minus (64 + z); the other four the same from w >> 8: 9 operations for
-// 8 weights.  x comes in the same order of pairs, four v_perm_b32 for 8 values.
-// Codes to bfloat16: v_cvt_off_f32_i4 makes (q - 8) / 16 of a nibble, whose upper half is the bfloat16: 14 operations for
-// 8 weights.  Zero points other than 8 come in by sums of x (a product with ones): s (8 - z) sum x.
+// Codes to numbers: 16 + q has q as the upper four bits of its fraction.  A byte b holds two codes; b * (1 + 2^12), shifted
+// to the fraction by the same multiplication, has both in place, one in each half; and-or cuts them out and puts the
+// exponents in: two operations for two weights, of which the multiplication picks the byte by itself.  The 16 and the
+// zero point leave by the sum of x, a product of the same operand with ones:  sum (16 + q) x - (16 + z) sum x.  (Numbers of
+// 16 to 31 where -8 to 7 are meant cost five times the rounding of a float32 sum; exact codes, -8 to 7 by v_cvt_off_f32_i4 or
+// by half arithmetic, took 12 to 14 operations for 8 weights in place of 8 and the time was theirs.)
 // float32 x: three bfloat16 parts (8 + 8 + 8 bits, exact), three instructions.
 #include "block_ops.h"
 
 namespace qcnn {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef u32x4 u32x4_any __attribute__((aligned(1)));
 
@@ -42,14 +42,9 @@ struct XForm<float> {
     static constexpr int RAW = 2, PARTS = 3;
 };
 
-__device__ __forceinline__ u32x4 perm4(u32x4 v)  // elements (0,4) (1,5) (2,6) (3,7)
-{
-    return u32x4{__builtin_amdgcn_perm(v[2], v[0], 0x05040100), __builtin_amdgcn_perm(v[2], v[0], 0x07060302),
-                 __builtin_amdgcn_perm(v[3], v[1], 0x05040100), __builtin_amdgcn_perm(v[3], v[1], 0x07060302)};
-}
 __device__ __forceinline__ unsigned upper_halves(unsigned lo, unsigned hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302); }
 
-__device__ __forceinline__ void x_operand(f16_t, const u32x4 *raw, u32x4 *out) { out[0] = perm4(raw[0]); }
+__device__ __forceinline__ void x_operand(f16_t, const u32x4 *raw, u32x4 *out) { out[0] = raw[0]; }
 __device__ __forceinline__ void x_operand(bf16_t, const u32x4 *raw, u32x4 *out) { out[0] = raw[0]; }
 __device__ __forceinline__ void x_operand(float, const u32x4 *raw, u32x4 *out)
 {
@@ -69,53 +64,40 @@ __device__ __forceinline__ void x_operand(float, const u32x4 *raw, u32x4 *out)
     }
 }
 
-// (v & mask) | magic and the conversion of nibble 0 of byte B, one instruction each (the compiler makes two of both)
+// (byte B of v) * by
+template <int B>
+__device__ __forceinline__ unsigned byte_times(unsigned v, unsigned by)
+{
+    unsigned o;
+    if constexpr (B == 0) asm("v_mul_u32_u24_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0 src1_sel:DWORD" : "=v"(o) : "v"(v), "v"(by));
+    if constexpr (B == 1) asm("v_mul_u32_u24_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1 src1_sel:DWORD" : "=v"(o) : "v"(v), "v"(by));
+    if constexpr (B == 2) asm("v_mul_u32_u24_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2 src1_sel:DWORD" : "=v"(o) : "v"(v), "v"(by));
+    if constexpr (B == 3) asm("v_mul_u32_u24_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3 src1_sel:DWORD" : "=v"(o) : "v"(v), "v"(by));
+    return o;
+}
 __device__ __forceinline__ unsigned and_or(unsigned v, unsigned mask, unsigned magic)
 {
     unsigned o;
     asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(o) : "v"(v), "s"(mask), "v"(magic));
     return o;
 }
-template <int B>
-__device__ __forceinline__ unsigned sixteenths(unsigned v)
-{
-    unsigned o;
-    if constexpr (B == 0) asm("v_cvt_off_f32_i4_e32 %0, %1" : "=v"(o) : "v"(v));
-    if constexpr (B == 1) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(o) : "v"(v));
-    if constexpr (B == 2) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(o) : "v"(v));
-    if constexpr (B == 3) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(o) : "v"(v));
-    return o;
-}
 
-// 8 codes of a dword as the other operand; z: the pair of constants of a half operand (unused otherwise)
-struct HalfZero {
-    f16x2 low, high;  // -(1024 + z), -(64 + z)
+// The 8 codes of a dword as 16 + q, and the ones that go with them
+template <typename T>
+struct Codes {  // bfloat16, for float32 x too
+    static constexpr unsigned BY = 1 << 3 | 1 << 15, MASK = 0x00780078, MAGIC = 0x41804180, ONES = 0x3f803f80;
 };
-__device__ __forceinline__ HalfZero half_zero(float z)
+template <>
+struct Codes<f16_t> {
+    static constexpr unsigned BY = 1 << 6 | 1 << 18, MASK = 0x03c003c0, MAGIC = 0x4c004c00, ONES = 0x3c003c00;
+};
+template <typename T>
+__device__ __forceinline__ u32x4 codes(unsigned w)
 {
-    const f16_t a = (f16_t)(-1024.f - z), b = (f16_t)(-64.f - z);
-    return HalfZero{f16x2{a, a}, f16x2{b, b}};
+    typedef Codes<T> C;
+    return u32x4{and_or(byte_times<0>(w, C::BY), C::MASK, C::MAGIC), and_or(byte_times<1>(w, C::BY), C::MASK, C::MAGIC),
+                 and_or(byte_times<2>(w, C::BY), C::MASK, C::MAGIC), and_or(byte_times<3>(w, C::BY), C::MASK, C::MAGIC)};
 }
-__device__ __forceinline__ u32x4 codes(f16_t, unsigned w, const HalfZero &z)
-{
-    const f16x2 r = {(f16_t)0.0625f, (f16_t)0.0625f};
-    u32x4 o;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const unsigned v = h ? w >> 8 : w;
-        const f16x2 a = __builtin_bit_cast(f16x2, and_or(v, 0x000f000fu, 0x64006400u)), b = __builtin_bit_cast(f16x2, and_or(v, 0x00f000f0u, 0x64006400u));
-        o[2 * h] = __builtin_bit_cast(unsigned, (f16x2)(a + z.low));
-        o[2 * h + 1] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(b, r, z.high));
-    }
-    return o;
-}
-__device__ __forceinline__ u32x4 codes(bf16_t, unsigned w, const HalfZero &)
-{
-    const unsigned even = w ^ 0x88888888u, odd = even >> 4;  // two's complement of q - 8
-    return u32x4{upper_halves(sixteenths<0>(even), sixteenths<0>(odd)), upper_halves(sixteenths<1>(even), sixteenths<1>(odd)),
-                 upper_halves(sixteenths<2>(even), sixteenths<2>(odd)), upper_halves(sixteenths<3>(even), sixteenths<3>(odd))};
-}
-__device__ __forceinline__ u32x4 codes(float, unsigned w, const HalfZero &z) { return codes(bf16_t(), w, z); }
 
 __device__ __forceinline__ f32x4 mma(f16_t, u32x4 x, u32x4 w, f32x4 c)
 {
@@ -160,27 +142,41 @@ __device__ __forceinline__ const char *uniform(const char *p)
     return (const char *)((unsigned long long)hi << 32 | lo);
 }
 
+// Waits until at most min(runs, MOST) runs' loads, and nothing else, are on their way.
+template <int MOST, int LOADS>
+__device__ __forceinline__ void wait_for_all_but(int runs)
+{
+    if constexpr (MOST <= 0) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    } else {
+        if (runs >= MOST)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * MOST) : "memory");
+        else
+            wait_for_all_but<MOST - 1, LOADS>(runs);
+    }
+}
+
 // LDS of one run of 128 k: x of XROWS rows for the NW waves, then for each wave its codes (1 KB a tile of 16 outputs) and
 // the scales and zero points of its outputs, a dword each, one set for FL instructions.  Chunk c of 16 bytes of x row r stands in slot c ^ (r & 15) of
 // its row: the sixteen lanes that a ds_read_b128 serves at a time read different slots of the 256 bytes that the banks hold.
-template <typename T, int NT, int XROWS, int FL, bool S16, bool ZERO, int KW, int NW, int R>
+template <typename T, int NT, int XROWS, int FL, bool S16, bool ZERO, int KW, int NW, int KB>
 struct W4 {
     static constexpr int WAVES = KW * NW, MT = XROWS < 16 ? 1 : XROWS / 16;
     static constexpr int XB = XROWS * 128 * (int)sizeof(T), NS = 4 / FL, SB = NS * NT * 64, SI = (SB + 255) / 256;
     static constexpr int WB = NT * 1024 + SI * 256 * (ZERO ? 2 : 1), RUN = XB + NW * WB;
     static constexpr int LOADS = NT + XB / 1024 / NW + SI * (ZERO ? 2 : 1);  // direct loads of a wave for one run
+    static constexpr int FIT = KB * 1024 / (KW * RUN), R = FIT < 2 ? 2 : FIT < 8 ? FIT : 8;  // runs in the ring: as many as KB kilobytes hold
     static constexpr int SUMS = WAVES * NT * MT * 1024;
     static constexpr int LDS = KW * R * RUN > SUMS ? KW * R * RUN : SUMS;
     static_assert(XB / 1024 % NW == 0 && NT <= 4 && LOADS * (R - 2) < 64 && LDS <= 163840, "runs fit");
 };
 
 // S16: scales of 16 bits; ZERO: zero points are given.
-template <typename T, int NT, int XROWS, int FL, bool S16, bool ZERO, int KW, int NW, int R>
+template <typename T, int NT, int XROWS, int FL, bool S16, bool ZERO, int KW, int NW, int KB>
 __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, unsigned nblocks)
 {
-    typedef W4<T, NT, XROWS, FL, S16, ZERO, KW, NW, R> G;
-    constexpr int PARTS = XForm<T>::PARTS, RAW = XForm<T>::RAW, MT = G::MT, NS = G::NS, TS = sizeof(T), SS = S16 ? 2 : 4;
-    constexpr bool HALF = __is_same(T, f16_t);
+    typedef W4<T, NT, XROWS, FL, S16, ZERO, KW, NW, KB> G;
+    constexpr int PARTS = XForm<T>::PARTS, RAW = XForm<T>::RAW, MT = G::MT, NS = G::NS, R = G::R, TS = sizeof(T), SS = S16 ? 2 : 4;
     extern __shared__ __align__(1024) char lds[];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
@@ -205,80 +201,108 @@ __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, un
         const int at = (i * NW + nq) * 64 + lane, row = at / CPR;
         xat[i] = (unsigned)min(row, rows - 1) * (unsigned)(a.ldx * TS) + ((at % CPR) ^ (row & 15)) * 16;
     }
-    // scale e = 64 i + lane of a run: of set e / 16 NT, output e % 16 NT
-    unsigned col[G::SI];
+    const int nbase = min(n0, a.n - 1);  // (a wave beyond the outputs reads the last one's and stores nothing)
+    const unsigned per = (unsigned)a.group >> 5;  // 32s of k in a group
+    char *const ring = lds + kq * (R * G::RUN);
+    const unsigned ring_at = (unsigned)(size_t)(__attribute__((address_space(3))) char *)ring;
+
+    // What moves from run to run, in scalar registers: a wave has few companions to hide a long scalar sum behind.
+    const char *w = uniform((const char *)a.w + (size_t)nbase * a.ldw + (size_t)first * 64);
+    const char *x = uniform((const char *)a.x + ((size_t)m0 * a.ldx + (size_t)first * 128) * TS);
+    const unsigned group = (unsigned)first * 4 / per;
+    unsigned used = (unsigned)first * 4 % per;  // 32s of k of the next run's group that are behind us
+    const char *sc = uniform((const char *)a.scale + ((size_t)group * a.n + nbase) * SS);
+    const char *zp = uniform((const char *)a.zero + (size_t)group * a.n + nbase);
+    int bring_slot = 0;
+    // Scale e = 64 i + lane of a run is that of set e / 16 NT, output e % 16 NT.  With groups of 32, 64 or whole 128s the sets of
+    // every run lie at the same distances (n <= 2^26: they fit).
+    const bool steady = FL == 4 || per <= 2;
+    unsigned col[G::SI], offset[G::SI];
     int set[G::SI];
 #pragma unroll
     for (int i = 0; i < G::SI; ++i) {
         set[i] = min((i * 64 + lane) / (16 * NT), NS - 1);
         col[i] = (unsigned)max(0, min((i * 64 + lane) % (16 * NT), a.n - 1 - n0));
+        offset[i] = col[i] + (FL == 4 ? 0u : (unsigned)(set[i] * FL) / per * (unsigned)a.n);
     }
-    const int nbase = min(n0, a.n - 1);  // (a wave beyond the outputs reads the last one's and stores nothing)
-    const char *const w0 = (const char *)a.w + (size_t)nbase * a.ldw, *const x0 = (const char *)a.x + (size_t)m0 * a.ldx * TS;
-    const unsigned per = (unsigned)a.group >> 5, last = (unsigned)(a.k - 1) / (unsigned)a.group;
-    char *const ring = lds + kq * (R * G::RUN);
-    const unsigned ring_at = (unsigned)(size_t)(__attribute__((address_space(3))) char *)ring;
-
-    unsigned gi = (unsigned)first * 4 / per, left = per - (unsigned)first * 4 % per;  // group of the next run to bring, its 32s of k left
-    const auto next_scales = [&](size_t &from, unsigned (&offset)[G::SI]) {  // elements: of the first set, and of each lane's from there
-        unsigned group[NS];
+    const auto sets_of_run = [&] {  // offset[] where they do not
+        unsigned step[NS], u = used, d = 0;
 #pragma unroll
         for (int f = 0; f < NS; ++f) {
-            group[f] = min(gi, last);  // (behind the last group x is zero)
-            left -= FL;
-            if (left == 0) ++gi, left = per;
+            step[f] = d;
+            u += FL;
+            if (u == per) u = 0, ++d;
         }
-        from = (size_t)group[0] * a.n + nbase;
 #pragma unroll
         for (int i = 0; i < G::SI; ++i) {
-            offset[i] = col[i];
+            unsigned by = 0;
 #pragma unroll
             for (int f = 1; f < NS; ++f)
-                if (set[i] == f) offset[i] += (group[f] - group[0]) * (unsigned)a.n;  // (n <= 2^26)
+                if (set[i] == f) by = step[f];
+            offset[i] = col[i] + by * (unsigned)a.n;
         }
     };
-    // brings run i (of this group) into the ring
+    // brings run i (of this group) into the ring; called for 0, 1, 2 ...
     const auto bring = [&](int i) {
-        const int kb = first + i, slot = i % R;
         if (i < whole) {
-            const unsigned at = ring_at + slot * G::RUN, mine = at + G::XB + nq * G::WB;
-            const char *w = uniform(w0 + (size_t)kb * 64), *x = uniform(x0 + (size_t)kb * (128 * TS));
+            const unsigned at = ring_at + bring_slot, mine = at + G::XB + nq * G::WB;
 #pragma unroll
             for (int t = 0; t < NT; ++t) lds_load16(mine + t * 1024, wat[t], w);
 #pragma unroll
             for (int j = 0; j < G::XB / 1024 / NW; ++j) lds_load16(at + (j * NW + nq) * 1024, xat[j], x);
-            size_t from;
-            unsigned offset[G::SI];
-            next_scales(from, offset);
+            if (!steady) sets_of_run();
 #pragma unroll
             for (int j = 0; j < G::SI; ++j) {
-                lds_load_one<SS>(mine + NT * 1024 + j * 256, offset[j] * SS, uniform((const char *)a.scale + from * SS));
-                if (ZERO) lds_load_one<1>(mine + NT * 1024 + (G::SI + j) * 256, offset[j], uniform((const char *)a.zero + from));
+                lds_load_one<SS>(mine + NT * 1024 + j * 256, offset[j] * SS, sc);
+                if (ZERO) lds_load_one<1>(mine + NT * 1024 + (G::SI + j) * 256, offset[j], zp);
+            }
+            w += 64;
+            x += 128 * TS;
+            used += 4;
+            while (used >= per) {  // (at most four times)
+                used -= per;
+                sc += (size_t)a.n * SS;
+                zp += a.n;
             }
         } else if (cut && i == whole) {  // element by element, zeros behind the end of x
-            char *at = ring + slot * G::RUN, *mine = at + G::XB + nq * G::WB;
-            for (int e = lane; e < NT * 1024; e += 64) {  // byte e & 63 of weight row e >> 6; lane (row & 15) + 16 (byte >> 4) reads it
-                const int row = e >> 6, byte = e & 63;
-                mine[(row >> 4) * 1024 + ((byte >> 4) * 16 + (row & 15)) * 16 + (byte & 15)] =
-                    kb * 64 + byte < row_bytes && n0 + row < a.n ? w0[(size_t)row * a.ldw + kb * 64 + byte] : 0;
+            const int kb = first + i;
+            char *at = ring + bring_slot, *mine = at + G::XB + nq * G::WB;
+            // (eight loads on their way at a time: 5 x 1001 x 2047 float32 took 12.5 us with one, 10.7 with eight)
+#pragma unroll 1
+            for (int t = 0; t < 2 * NT; ++t) {  // of 8 rows the lane brings byte lane; lane (row + 16 (byte >> 4)) of their tile reads it
+                uint8_t v[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) v[r] = kb * 64 + lane < row_bytes && n0 + t * 8 + r < a.n ? w[(size_t)(t * 8 + r) * a.ldw + lane] : 0;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) mine[(t >> 1) * 1024 + ((lane >> 4) * 16 + (t & 1) * 8 + r) * 16 + (lane & 15)] = v[r];
             }
-            T zero;
-            from_f32(0.f, zero);
-            for (int e = nq * 64 + lane; e < XROWS * 128; e += NW * 64) {
-                const int row = e >> 7, k = e & 127, c = k * TS / 16;
-                *(T *)(at + row * (128 * TS) + (c ^ (row & 15)) * 16 + k * TS % 16) =
-                    kb * 128 + k < a.k ? ((const T *)x0)[(size_t)min(row, rows - 1) * a.ldx + kb * 128 + k] : zero;
+            constexpr int EACH = XROWS * 128 / (NW * 64), BATCH = EACH < 8 ? EACH : 8;
+            static_assert(XROWS * 128 % (NW * 64) == 0 && EACH % BATCH == 0, "whole batches");
+#pragma unroll 1
+            for (int e0 = 0; e0 < EACH; e0 += BATCH) {
+                T v[BATCH];
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    const int e = ((e0 + i) * NW + nq) * 64 + lane, row = e >> 7, k = e & 127;
+                    from_f32(0.f, v[i]);
+                    if (kb * 128 + k < a.k) v[i] = ((const T *)x)[(size_t)min(row, rows - 1) * a.ldx + k];
+                }
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    const int e = ((e0 + i) * NW + nq) * 64 + lane, row = e >> 7, k = e & 127, c = k * TS / 16;
+                    *(T *)(at + row * (128 * TS) + (c ^ (row & 15)) * 16 + k * TS % 16) = v[i];
+                }
             }
-            size_t from;
-            unsigned offset[G::SI];
-            next_scales(from, offset);
+            const unsigned last = (unsigned)(a.k - 1) / (unsigned)a.group;  // (behind the last group x is zero)
 #pragma unroll
             for (int j = 0; j < G::SI; ++j) {
+                const size_t e = (size_t)min(((unsigned)kb * 4 + set[j] * FL) / per, last) * a.n + nbase + col[j];
                 unsigned *sz = (unsigned *)(mine + NT * 1024 + j * 256) + lane;
-                *sz = S16 ? ((const uint16_t *)a.scale)[from + offset[j]] : ((const unsigned *)a.scale)[from + offset[j]];
-                if (ZERO) sz[G::SI * 64] = ((const uint8_t *)a.zero)[from + offset[j]];
+                *sz = S16 ? ((const uint16_t *)a.scale)[e] : ((const unsigned *)a.scale)[e];
+                if (ZERO) sz[G::SI * 64] = ((const uint8_t *)a.zero)[e];
             }
         }
+        bring_slot = bring_slot == (R - 1) * G::RUN ? 0 : bring_slot + G::RUN;
     };
 
     f32x4 acc[NT][MT];
@@ -288,28 +312,41 @@ __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, un
         for (int m = 0; m < MT; ++m) acc[t][m] = f32x4{0, 0, 0, 0};
     const bool bf16_scales = a.scale_type == QCNN_BF16;
 
-    const auto consume = [&](int i) {
-        const char *at = ring + i % R * G::RUN, *mine = at + G::XB + nq * G::WB;
-        u32x4 w[NT];
+    // a run in registers: everything is asked of LDS before the first of it is used
+    struct Run {
+        u32x4 w[NT], x[4][MT][RAW];
+        unsigned s[NS][NT], z[NS][NT];
+    };
+    int slot = 0;
+    const auto fetch = [&](Run &r) {
+        const char *at = ring + slot, *mine = at + G::XB + nq * G::WB;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) w[t] = transpose4(*(const u32x4 *)(mine + t * 1024 + lane * 16));
+        for (int t = 0; t < NT; ++t) r.w[t] = *(const u32x4 *)(mine + t * 1024 + lane * 16);
 #pragma unroll
-        for (int f = 0; f < NS; ++f) {
-            f32x4 sum[NT][MT], ones[MT];
-            float s[NT], z[NT];
-            HalfZero hz[NT];
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const int row = XROWS < 16 ? c16 % XROWS : m * 16 + c16;
+#pragma unroll
+                for (int i = 0; i < RAW; ++i) r.x[j][m][i] = *(const u32x4 *)(at + row * (128 * TS) + (((j * 4 + g) * RAW + i) ^ (row & 15)) * 16);
+            }
+#pragma unroll
+        for (int f = 0; f < NS; ++f)
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const char *p = mine + NT * 1024 + (f * 16 * NT + t * 16 + c16) * 4;
-                if (S16) {
-                    const unsigned u = *(const uint16_t *)p;
-                    s[t] = bf16_scales ? __uint_as_float(u << 16) : (float)__builtin_bit_cast(f16_t, (uint16_t)u);
-                } else {
-                    s[t] = *(const float *)p;
-                }
-                z[t] = ZERO ? (float)*(const uint8_t *)(p + G::SI * 256) : 8.f;
-                hz[t] = half_zero(z[t]);
+                r.s[f][t] = S16 ? *(const uint16_t *)p : *(const unsigned *)p;
+                if (ZERO) r.z[f][t] = *(const uint8_t *)(p + G::SI * 256);
             }
+        slot = slot == (R - 1) * G::RUN ? 0 : slot + G::RUN;
+    };
+    const auto compute = [&](const Run &r) {
+        u32x4 w[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) w[t] = transpose4(r.w[t]);
+#pragma unroll
+        for (int f = 0; f < NS; ++f) {
+            f32x4 sum[NT][MT], ones[MT];
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 ones[m] = f32x4{0, 0, 0, 0};
@@ -321,21 +358,14 @@ __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, un
                 u32x4 x[MT][PARTS];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    const int row = XROWS < 16 ? c16 % XROWS : m * 16 + c16;
-                    u32x4 raw[RAW];
+                    x_operand(T(), r.x[j][m], x[m]);
+                    const u32x4 one = {Codes<T>::ONES, Codes<T>::ONES, Codes<T>::ONES, Codes<T>::ONES};
 #pragma unroll
-                    for (int r = 0; r < RAW; ++r)
-                        raw[r] = *(const u32x4 *)(at + row * (128 * TS) + (((j * 4 + g) * RAW + r) ^ (row & 15)) * 16);
-                    x_operand(T(), raw, x[m]);
-                    if (!HALF && ZERO) {
-                        const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-#pragma unroll
-                        for (int p = 0; p < PARTS; ++p) ones[m] = mma(T(), x[m][p], one, ones[m]);
-                    }
+                    for (int p = 0; p < PARTS; ++p) ones[m] = mma(T(), x[m][p], one, ones[m]);
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const u32x4 c = codes(T(), w[t][j], hz[t]);
+                    const u32x4 c = codes<T>(w[t][j]);
 #pragma unroll
                     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -344,33 +374,30 @@ __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, un
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const float s16 = HALF ? s[t] : 16.f * s[t], sz = s[t] * (8.f - z[t]);
+                const unsigned u = r.s[f][t];
+                const float s = !S16 ? __uint_as_float(u) : bf16_scales ? __uint_as_float(u << 16) : (float)__builtin_bit_cast(f16_t, (uint16_t)u);
+                const float z = 16.f + (ZERO ? (float)r.z[f][t] : 8.f);
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        acc[t][m][q] = fmaf(s16, sum[t][m][q], acc[t][m][q]);
-                        if (!HALF && ZERO) acc[t][m][q] = fmaf(sz, ones[m][q], acc[t][m][q]);
-                    }
+                    for (int q = 0; q < 4; ++q) acc[t][m][q] = fmaf(s, fmaf(-z, ones[m][q], sum[t][m][q]), acc[t][m][q]);
             }
         }
     };
 
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < R - 1; ++i) bring(i);
     for (int i = 0; i < turns; ++i) {
-        // run i has landed (loads land in order: all but those of the runs behind it), here and after the barrier for all,
-        // and everyone is done with run i - 1, whose place run i + R - 1 takes
-        const int behind = min(R - 2, whole - 1 - i);
-        if (R > 3 && behind >= 2)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(G::LOADS * 2) : "memory");
-        else if (R > 2 && behind >= 1)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(G::LOADS) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        // run i has landed (loads land in order: all but those of the runs behind it), here and after the barrier for all, and
+        // everyone is done with run i - 1, whose place run i + R - 1 takes
+        wait_for_all_but<R - 2, G::LOADS>(whole - 1 - i);
         if (NW > 1) asm volatile("s_barrier" ::: "memory");
         bring(i + R - 1);
-        if (i < count) consume(i);
+        if (i < count) {
+            Run r;
+            fetch(r);
+            compute(r);
+        }
     }
 
     // the k groups' sums; the lane has rows 4 g .. 4 g + 3 of output c16 of each tile
@@ -396,14 +423,14 @@ __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, un
     }
 }
 
-template <typename T, int NT, int XROWS, int FL, bool S16, bool ZERO, int KW, int NW, int R>
+template <typename T, int NT, int XROWS, int FL, bool S16, bool ZERO, int KW, int NW, int KB>
 static hipError_t launch(const qcnn_matvec_w4_t &a, hipStream_t s)
 {
-    typedef W4<T, NT, XROWS, FL, S16, ZERO, KW, NW, R> G;
+    typedef W4<T, NT, XROWS, FL, S16, ZERO, KW, NW, KB> G;
     const unsigned nblocks = (unsigned)((a.n + 16 * NT * NW - 1) / (16 * NT * NW));
     const unsigned long long blocks = (unsigned long long)nblocks * ((a.rows + XROWS - 1) / XROWS);
     if (blocks * (64 * G::WAVES) > 0xffffffffull) return hipErrorInvalidConfiguration;
-    const auto fn = k_w4<T, NT, XROWS, FL, S16, ZERO, KW, NW, R>;
+    const auto fn = k_w4<T, NT, XROWS, FL, S16, ZERO, KW, NW, KB>;
     if (G::LDS > 65536) {
         const hipError_t e = hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
         if (e != hipSuccess) return e;
@@ -412,21 +439,36 @@ static hipError_t launch(const qcnn_matvec_w4_t &a, hipStream_t s)
     return hipGetLastError();
 }
 
-template <typename T, int NT, int XROWS, int FL, int KW, int NW, int R>
+template <typename T, int NT, int XROWS, int FL, int KW, int NW, int KB>
 static hipError_t run(const qcnn_matvec_w4_t &a, hipStream_t s)
 {
     if (a.scale_type != QCNN_F32)
-        return a.zero ? launch<T, NT, XROWS, FL, true, true, KW, NW, R>(a, s) : launch<T, NT, XROWS, FL, true, false, KW, NW, R>(a, s);
-    return a.zero ? launch<T, NT, XROWS, FL, false, true, KW, NW, R>(a, s) : launch<T, NT, XROWS, FL, false, false, KW, NW, R>(a, s);
+        return a.zero ? launch<T, NT, XROWS, FL, true, true, KW, NW, KB>(a, s) : launch<T, NT, XROWS, FL, true, false, KW, NW, KB>(a, s);
+    return a.zero ? launch<T, NT, XROWS, FL, false, true, KW, NW, KB>(a, s) : launch<T, NT, XROWS, FL, false, false, KW, NW, KB>(a, s);
 }
 
+// Rows of x a workgroup takes and how its waves share out the work.  With few outputs there are few workgroups, each
+// wave is alone with its instructions' latencies, and more waves along k are what helps; with many outputs, sharing x
+// among waves and several workgroups on a CU.  Microseconds at k = 4096, cold memory, group 128, for n = 1024 / 4096 / 8192 /
+// 16384, the taken side of each border first:
+//   bfloat16 rows <= 4     4.6 / 4.9 / 7.2 / 11.0   (KB 80: 4.7 / 5.4 / 7.6 / 12.9;  two tiles a wave 6.1 / 6.3 / 7.4 / 10.8)
+//            rows <= 16    8 x 1 5.5 / 6.4 / 12.0 / 21.9 up to 4096, 4 x 2 7.6 / 8.1 / 9.1 / 14.2 above
+//            rows <= 64    32 rows 4 x 2 9.5 / 11.0 / 20.4 / 40.1 up to 4096, 64 rows 2 x 4 20.5 / 22.4 / 23.0 / 26.8 above
+//   float32  rows <= 4     one tile 7.4 / 8.1 / 13.5 / 22.9 up to 4096, two 8.6 / 9.2 / 10.2 / 16.9 above
+//            rows <= 16    one tile 13.1 / 14.1 / 15.5 / 30.1 up to 8192, two 17.2 / 18.5 / 19.5 / 21.8 above
+//            rows <= 64    16 rows 4 x 4 20.5 / 24.1 / 44.4 / 96.1 up to 4096, 32 rows, two tiles 47.2 / 49.4 / 49.7 / 60.1 above
 template <typename T, int FL>
 static hipError_t pick_rows(const qcnn_matvec_w4_t &a, hipStream_t s)
 {
-    constexpr bool F = sizeof(T) == 4;
-    if (a.rows > 16) return run<T, 1, F ? 32 : 64, FL, 2, 4, 3>(a, s);
-    if (a.rows > 4) return run<T, 1, 16, FL, 2, 4, F ? 3 : 4>(a, s);
-    return run<T, 1, 4, FL, 8, 1, FL == 1 ? 3 : 4>(a, s);
+    if constexpr (sizeof(T) == 4) {
+        if (a.rows <= 4) return a.n <= 4096 ? run<T, 1, 4, FL, 8, 1, 80>(a, s) : run<T, 2, 4, FL, 8, 1, 80>(a, s);
+        if (a.rows <= 16) return a.n <= 8192 ? run<T, 1, 16, FL, 4, 2, 80>(a, s) : run<T, 2, 16, FL, 4, 2, 160>(a, s);
+        return a.n <= 4096 ? run<T, 1, 16, FL, 4, 4, 160>(a, s) : run<T, 2, 32, FL, 2, 4, 160>(a, s);
+    } else {
+        if (a.rows <= 4) return run<T, 1, 4, FL, 8, 1, 53>(a, s);
+        if (a.rows <= 16) return a.n <= 4096 ? run<T, 1, 16, FL, 8, 1, 160>(a, s) : run<T, 1, 16, FL, 4, 2, 80>(a, s);
+        return a.n <= 4096 ? run<T, 1, 32, FL, 4, 2, 160>(a, s) : run<T, 1, 64, FL, 2, 4, 160>(a, s);
+    }
 }
 
 template <typename T>
