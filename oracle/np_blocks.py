@@ -50,25 +50,26 @@ def grouped_matmul(x, w, offsets, src, x_scale, w_scale, bias, row_scale, act, y
     w8, x8 = w.astype(np.float64), x.astype(np.float64)
     for e in range(experts):
         lo, hi = max(0, int(offsets[e])), min(rows, int(offsets[e + 1]))
-        for r in range(lo, hi):
-            s = r if src is None else int(src[r])
-            have = 0 <= s < x.shape[0]
-            xv = x8[s] if have else np.zeros(k)
-            v, size = w8[e] @ xv, np.abs(w8[e]) @ np.abs(xv)
-            if x.dtype == np.int8:
-                size = np.abs(v) * 4 / (k + 8)  # exact sums, one rounding to float32
-            for f in (w_scale[e] if w_scale is not None else None, x_scale[s] if x_scale is not None and have else None):
-                if f is not None:
-                    f = np.asarray(f, np.float64)
-                    v, size = v * f, size * np.abs(f)
-            if bias is not None:
-                v, size = v + bias[e], size + np.abs(bias[e])
-            b = 2 * (k + 8) * U * size
-            if act == 2:  # |silu'| <= 1.1; e^-v in float32 is off by a few U relative, more where |v| is large
-                b = 1.1 * b + (8 + np.abs(v)) * 2 * U * np.abs(act_of(v, 2))
-            v = act_of(v, act)
-            f = 1.0 if row_scale is None else float(row_scale[r])
-            out[r], bound[r] = v * f, (b + 2 * U * np.abs(v)) * abs(f)
+        if lo >= hi:
+            continue
+        s = np.arange(lo, hi) if src is None else src[lo:hi].astype(np.int64)
+        have = (s >= 0) & (s < x.shape[0])
+        at = np.where(have, s, 0)
+        xv = np.where(have[:, None], x8[at], 0) if x.shape[0] else np.zeros((hi - lo, k))
+        v, size = xv @ w8[e].T, np.abs(xv) @ np.abs(w8[e]).T
+        if x.dtype == np.int8:
+            size = np.abs(v) * 4 / (k + 8)  # exact sums, one rounding to float32
+        for f in (w_scale[e][None, :] if w_scale is not None else None, np.where(have, x_scale[at], 1)[:, None] if x_scale is not None else None):
+            if f is not None:
+                v, size = v * f.astype(np.float64), size * np.abs(f.astype(np.float64))
+        if bias is not None:
+            v, size = v + bias[e], size + np.abs(bias[e])
+        b = 2 * (k + 8) * U * size
+        if act == 2:  # |silu'| <= 1.1; e^-v in float32 is off by a few U relative, more where |v| is large
+            b = 1.1 * b + (8 + np.abs(v)) * 2 * U * np.abs(act_of(v, 2))
+        v = act_of(v, act)
+        f = np.ones((hi - lo, 1)) if row_scale is None else row_scale[lo:hi].astype(np.float64)[:, None]
+        out[lo:hi], bound[lo:hi] = v * f, (b + 2 * U * np.abs(v)) * np.abs(f)
     return out, bound
 
 

@@ -5,6 +5,7 @@
 namespace qcnn {
 
 typedef u32x4 u32x4_any __attribute__((aligned(1)));  // global loads and stores take any address
+typedef u32x2 u32x2_any __attribute__((aligned(1)));
 
 // 16 bytes of a row are a chunk; a matrix instruction of 16 x 16 outputs takes a chunk of every lane: lane l holds
 // chunk (l >> 4) of four of row l & 15.  Both operands come in the same order, so the order of k inside a chunk is free:
@@ -12,10 +13,12 @@ typedef u32x4 u32x4_any __attribute__((aligned(1)));  // global loads and stores
 template <typename T>
 struct Mma {
     typedef f32x4 acc_t;
+    typedef float one_t;
 };
 template <>
 struct Mma<int8_t> {
     typedef i32x4 acc_t;
+    typedef int one_t;
 };
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -122,11 +125,17 @@ __device__ __forceinline__ void store_row(const qcnn_grouped_matmul_t &a, const 
     for (int q = 0; q < N; ++q) from_f32((v[q] < least ? least : v[q]) * rs, o[q]);
     OT *y = (OT *)a.y + r * a.ldy + n;
     if (n + N <= a.n) {
-        constexpr int C = sizeof o / 16;
-        u32x4 c[C];
-        __builtin_memcpy(c, o, sizeof o);
+        if constexpr (sizeof o == 8) {
+            u32x2 c;
+            __builtin_memcpy(&c, o, 8);
+            *(u32x2_any *)y = c;
+        } else {
+            constexpr int C = sizeof o / 16;
+            u32x4 c[C];
+            __builtin_memcpy(c, o, sizeof o);
 #pragma unroll
-        for (int i = 0; i < C; ++i) ((u32x4_any *)y)[i] = c[i];
+            for (int i = 0; i < C; ++i) ((u32x4_any *)y)[i] = c[i];
+        }
     } else {
 #pragma unroll
         for (int q = 0; q < N - 1; ++q)
@@ -386,6 +395,175 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grou
     }
 }
 
+// ---- few rows an expert --------------------------------------------------------------------------------
+// Reading the weights is the cost.  A workgroup takes up to 16 MT rows of one expert and 16 NW outputs; its waves are
+// KW x NW, NW share out the outputs and KW the k, in runs of RB bytes, and the KW sums meet in LDS at the end.  Direct loads
+// bring the chunks in the order of the matrix instruction's lanes, R - 1 runs ahead: 1 KB of LDS is one operand, 64 bytes of
+// k of 16 rows.  x is shared by the NW waves of a k group (one barrier a run, none for NW = 1), and of sixteen rows
+// only those that there are ask for it.
+template <typename T, int MT, int RB, int KW, int NW, int KB>
+struct RowsGeom {
+    static constexpr int OPS = RB / 64, WAVES = KW * NW;
+    static constexpr int XB = MT * OPS * 1024, RUN = XB + NW * OPS * 1024;
+    static constexpr int XL = MT * OPS / NW, LOADS = OPS + XL;  // direct loads of a wave for one run
+    static constexpr int FIT = KB * 1024 / (KW * RUN), R = FIT < 2 ? 2 : FIT < 8 ? FIT : 8;  // runs in the ring: as many as KB kilobytes hold
+    static constexpr int SUMS = WAVES * MT * 1024;
+    static constexpr int LDS = KW * R * RUN > SUMS ? KW * R * RUN : SUMS;
+    static_assert(MT * OPS % NW == 0 && LOADS * (R - 2) < 64 && LDS <= 163840, "runs fit");
+};
+
+// Waits until at most min(runs, MOST) runs' loads, and nothing else, are on their way.
+template <int MOST, int LOADS>
+__device__ __forceinline__ void wait_for_all_but(int runs)
+{
+    if constexpr (MOST <= 0) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    } else {
+        if (runs >= MOST)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * MOST) : "memory");
+        else
+            wait_for_all_but<MOST - 1, LOADS>(runs);
+    }
+}
+
+template <typename T, int MT, int RB, int KW, int NW, int KB, bool ALIGNED>
+__global__ __launch_bounds__(64 * KW *NW) void k_grouped_rows(const qcnn_grouped_matmul_t a)
+{
+    typedef RowsGeom<T, MT, RB, KW, NW, KB> G;
+    typedef typename Mma<T>::acc_t acc_t;
+    typedef typename Mma<T>::one_t one_t;
+    constexpr int OPS = G::OPS, R = G::R;
+    extern __shared__ __align__(1024) char lds[];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
+    const int kq = wave / NW, nq = wave % NW;
+    Tiles<16 * MT, 16 * NW> tiles;
+    tiles.count(a);
+    Tile t{0, 0, 0, 0};
+    if (!tiles.get(a, blockIdx.x >> 3, t)) return;
+
+    // this lane's rows: one of w and, for each operand of x that this wave brings, one of x
+    const int bytes = a.k * (int)sizeof(T), all = (bytes + RB - 1) / RB, turns = (all + KW - 1) / KW;
+    const int first = kq * turns, count = max(0, min(turns, all - first));
+    const char *wp = (const char *)a.w + ((size_t)t.e * a.w_stride + (size_t)min(t.n0 + nq * 16 + c16, a.n - 1) * a.ldw) * sizeof(T) + (size_t)first * RB;
+    const char *xp[G::XL];
+    bool has[G::XL];
+#pragma unroll
+    for (int i = 0; i < G::XL; ++i) {
+        const int row = (i * NW + nq) / OPS * 16 + c16, r = t.first + min(row, t.count - 1), s = a.src ? a.src[r] : r;
+        has[i] = MT > 1 || row < t.count;  // (a load that no lane asks for would not be counted by the waits: one tile always has a row)
+        xp[i] = (const char *)a.x + (size_t)(s >= 0 && s < a.x_rows ? s : 0) * a.ldx * sizeof(T) + (size_t)first * RB;
+    }
+    char *const ring = lds + kq * (R * G::RUN);
+    const unsigned ring_at = (unsigned)(size_t)(__attribute__((address_space(3))) char *)ring;
+    int bring_slot = 0;
+    // brings run i (of this group) into the ring; called for 0, 1, 2 ...
+    const auto bring = [&](int i) {
+        if (i < count) {
+            const int left = bytes - (first + i) * RB - g * 16;  // bytes of the rows from this lane's first chunk on
+            if constexpr (ALIGNED) {
+                const unsigned at = ring_at + bring_slot;
+#pragma unroll
+                for (int o = 0; o < OPS; ++o) load_to_lds(o * 64 < left ? wp + o * 64 : (const char *)&k_zero_chunk, at + G::XB + (nq * OPS + o) * 1024);
+#pragma unroll
+                for (int j = 0; j < G::XL; ++j) {
+                    const int o = (j * NW + nq) % OPS;
+                    if (has[j]) load_to_lds(o * 64 < left ? xp[j] + o * 64 : (const char *)&k_zero_chunk, at + (j * NW + nq) * 1024);
+                }
+            } else {
+                char *at = ring + bring_slot + lane * 16;
+                u32x4 v[OPS + G::XL];
+#pragma unroll
+                for (int o = 0; o < OPS; ++o) v[o] = load_chunk(wp, o * 4, left);
+#pragma unroll
+                for (int j = 0; j < G::XL; ++j) v[OPS + j] = load_chunk(xp[j], (j * NW + nq) % OPS * 4, left);
+#pragma unroll
+                for (int o = 0; o < OPS; ++o) *(u32x4 *)(at + G::XB + (nq * OPS + o) * 1024) = v[o];
+#pragma unroll
+                for (int j = 0; j < G::XL; ++j) *(u32x4 *)(at + (j * NW + nq) * 1024) = v[OPS + j];
+            }
+            wp += RB;
+#pragma unroll
+            for (int j = 0; j < G::XL; ++j) xp[j] += RB;
+        }
+        bring_slot = bring_slot == (R - 1) * G::RUN ? 0 : bring_slot + G::RUN;
+    };
+    wp += g * 16;
+#pragma unroll
+    for (int j = 0; j < G::XL; ++j) xp[j] += g * 16;
+
+    acc_t acc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m] = acc_t{0, 0, 0, 0};
+    int slot = 0;
+#pragma unroll 1
+    for (int i = 0; i < R - 1; ++i) bring(i);
+    for (int i = 0; i < turns; ++i) {
+        // run i has landed (loads land in order: all but those of the runs behind it), here and after the barrier for all, and
+        // everyone is done with run i - 1, whose place run i + R - 1 takes
+        wait_for_all_but<R - 2, G::LOADS>(count - 1 - i);
+        if (NW > 1) asm volatile("s_barrier" ::: "memory");
+        bring(i + R - 1);
+        if (i < count) {
+            const char *at = ring + slot + lane * 16;
+            u32x4 w[OPS], x[OPS][MT];
+#pragma unroll
+            for (int o = 0; o < OPS; ++o) {
+                w[o] = *(const u32x4 *)(at + G::XB + (nq * OPS + o) * 1024);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) x[o][m] = *(const u32x4 *)(at + (m * OPS + o) * 1024);
+            }
+#pragma unroll
+            for (int o = 0; o < OPS; ++o)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) acc[m] = mma(T(), x[o][m], w[o], acc[m]);
+        }
+        slot = slot == (R - 1) * G::RUN ? 0 : slot + G::RUN;
+    }
+
+    // the k groups' sums; the lane has rows 4 g .. 4 g + 3 of output c16
+    __syncthreads();
+    one_t *sums = (one_t *)lds;
+    constexpr int OUT = 16 * NW;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sums[kq * (OUT * 16 * MT) + (m * 16 + 4 * g + q) * OUT + nq * 16 + c16] = acc[m][q];
+    __syncthreads();
+    for (int o = threadIdx.x; o < OUT * t.count; o += 64 * KW * NW) {
+        const int row = o / OUT, n = t.n0 + o % OUT;
+        if (n >= a.n) continue;
+        one_t v = 0;
+#pragma unroll
+        for (int k = 0; k < KW; ++k) v += sums[k * (OUT * 16 * MT) + o];
+        const int r = t.first + row, s = a.src ? a.src[r] : r;
+        const size_t e = (size_t)t.e * a.n + n;
+        float f = s >= 0 && s < a.x_rows ? (float)v : 0.f;
+        if (a.w_scale) f *= a.w_scale[e];
+        if (a.x_scale && s >= 0 && s < a.x_rows) f *= a.x_scale[s];
+        if (a.bias) f += a.bias[e];
+        f = block_act(f, a.act);
+        if (a.row_scale) f *= a.row_scale[r];
+        store_typed(a.y, (size_t)r * a.ldy + n, a.out_type, f);
+    }
+}
+
+template <typename T, int MT, int RB, int KW, int NW, int KB>
+static hipError_t run_rows(const qcnn_grouped_matmul_t &a, bool al, hipStream_t s)
+{
+    typedef RowsGeom<T, MT, RB, KW, NW, KB> G;
+    const unsigned long long tiles = (unsigned long long)most_tiles(a, 16 * MT) * ((a.n + 16 * NW - 1) / (16 * NW));
+    const unsigned long long blocks = (tiles + 7) / 8 * 8;  // as many on each XCD
+    if (blocks * (64 * KW * NW) > 0xffffffffull) return hipErrorInvalidConfiguration;
+    const auto fn = al ? k_grouped_rows<T, MT, RB, KW, NW, KB, true> : k_grouped_rows<T, MT, RB, KW, NW, KB, false>;
+    if (G::LDS > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
+        if (e != hipSuccess) return e;
+    }
+    fn<<<(unsigned)blocks, 64 * KW * NW, G::LDS, s>>>(a);
+    return hipGetLastError();
+}
+
 // Compute units of the current device, asked for once.
 static int compute_units()
 {
@@ -416,6 +594,90 @@ static hipError_t run_tile(const qcnn_grouped_matmul_t &a, bool al, hipStream_t 
     return hipGetLastError();
 }
 
+// ---- short rows and few outputs, many rows ---------------------------------------------------------------
+// Up to 64 outputs of rows of up to 256 bytes, the 1x1 layers of an image network: reading x and writing y is the cost.
+// A wave keeps the weights of all outputs in registers and runs over its rows, four tiles of sixteen at a time, straight
+// from memory into matrix instructions; four lanes write 64 bytes (float32) of a row side by side.
+template <typename T, int NT, int OPS>
+__global__ __launch_bounds__(256) void k_grouped_narrow(const qcnn_grouped_matmul_t a)
+{
+    typedef typename Mma<T>::acc_t acc_t;
+    constexpr int TM = 512, BATCH = OPS == 1 ? 4 : 2;  // rows of a workgroup; row tiles on their way at a time
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
+    Tiles<TM, 64> tiles;
+    tiles.count(a);
+    Tile t{0, 0, 0, 0};
+    if (!tiles.get(a, blockIdx.x >> 3, t)) return;
+
+    const int bytes = a.k * (int)sizeof(T);
+    u32x4 w[NT][OPS];
+    f32x4 ws[NT], b[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const char *row = (const char *)a.w + ((size_t)t.e * a.w_stride + (size_t)min(j * 16 + c16, a.n - 1) * a.ldw) * sizeof(T);
+#pragma unroll
+        for (int o = 0; o < OPS; ++o) w[j][o] = load_chunk(row, o * 4 + g, bytes);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const size_t n = (size_t)t.e * a.n + min(j * 16 + 4 * g + q, a.n - 1);
+            ws[j][q] = a.w_scale ? a.w_scale[n] : 1.f;
+            b[j][q] = a.bias ? a.bias[n] : 0.f;
+        }
+    }
+    const auto rows = [&](auto type) {
+        typedef decltype(type) OT;
+        const float least = a.act == QCNN_ACT_RELU ? 0.f : -__builtin_inff();
+        for (int m0 = wave * (TM / 4); m0 < min((wave + 1) * (TM / 4), t.count); m0 += 16 * BATCH) {
+            u32x4 x[BATCH][OPS];
+            float xs[BATCH], rs[BATCH];
+            bool have[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const int r = t.first + min(m0 + i * 16 + c16, t.count - 1), s = a.src ? a.src[r] : r;
+                have[i] = s >= 0 && s < a.x_rows;
+                const char *row = (const char *)a.x + (size_t)(have[i] ? s : 0) * a.ldx * sizeof(T);
+#pragma unroll
+                for (int o = 0; o < OPS; ++o) x[i][o] = load_chunk(row, o * 4 + g, bytes);
+                xs[i] = a.x_scale && have[i] ? a.x_scale[s] : 1.f;
+                rs[i] = a.row_scale ? a.row_scale[r] : 1.f;
+            }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const int m = m0 + i * 16 + c16;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    acc_t acc = {0, 0, 0, 0};
+#pragma unroll
+                    for (int o = 0; o < OPS; ++o) acc = mma(T(), w[j][o], x[i][o], acc);
+                    float v[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) v[q] = (have[i] ? (float)acc[q] * ws[j][q] * xs[i] : 0.f) + b[j][q];
+                    if (a.act == QCNN_ACT_SILU) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) v[q] = block_act(v[q], QCNN_ACT_SILU);
+                    }
+                    if (m < t.count && j * 16 + 4 * g < a.n) store_row<OT>(a, v, rs[i], least, (size_t)(t.first + m), j * 16 + 4 * g);
+                }
+            }
+        }
+    };
+    if (a.out_type == QCNN_F32)
+        rows(float());
+    else if (a.out_type == QCNN_F16)
+        rows(f16_t());
+    else
+        rows(bf16_t());
+}
+
+template <typename T, int NT, int OPS>
+static hipError_t run_narrow(const qcnn_grouped_matmul_t &a, hipStream_t s)
+{
+    const unsigned long long blocks = ((unsigned long long)most_tiles(a, 512) + 7) / 8 * 8;
+    if (blocks * 256 > 0xffffffffull) return hipErrorInvalidConfiguration;
+    k_grouped_narrow<T, NT, OPS><<<(unsigned)blocks, 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
 template <typename T>
 static hipError_t pick(qcnn_grouped_matmul_t a, hipStream_t s)
 {
@@ -423,8 +685,18 @@ static hipError_t pick(qcnn_grouped_matmul_t a, hipStream_t s)
     const size_t z = sizeof(T);
     const bool al = (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.w % 16 == 0 && a.ldx * z % 16 == 0 && a.ldw * z % 16 == 0 && a.w_stride * z % 16 == 0 &&
                     a.k * z % 16 == 0;
-    const long long tiles = (long long)a.rows * a.n / 65536;
-    if (tiles >= 256 && al && sizeof(T) < 4) return run_tile<T, 256, 256, 2, 4>(a, al, s);
+    // Which kernel, by the rows an expert has on average (the host does not know the offsets) and the tiles there can be.
+    const long long groups = a.rows < a.experts ? a.rows : a.experts, avg = a.rows / a.experts;
+    const auto tiles = [&](long long tm, long long tn) { return (a.rows / tm + groups) * ((a.n + tn - 1) / tn); };
+    if (a.n <= 64 && a.k * z <= 256 && avg >= 512) {
+        if (a.k * z <= 64) return a.n <= 32 ? run_narrow<T, 2, 1>(a, s) : run_narrow<T, 4, 1>(a, s);
+        return a.n <= 32 ? run_narrow<T, 2, 4>(a, s) : run_narrow<T, 4, 4>(a, s);
+    }
+    if (avg <= 4) return tiles(16, 32) < 256 ? run_rows<T, 1, 128, 8, 1, 80>(a, al, s) : run_rows<T, 1, 128, 4, 2, 80>(a, al, s);
+    if (tiles(64, 64) < 256) return run_rows<T, 2, 128, 4, 2, 80>(a, al, s);
+    if (avg <= 24) return run_rows<T, 4, 128, 2, 4, 80>(a, al, s);
+    if (tiles(128, 128) < 256) return run_tile<T, 64, 64, 2, 2>(a, al, s);
+    if (sizeof(T) < 4 && al && tiles(256, 256) >= 512) return run_tile<T, 256, 256, 2, 4>(a, al, s);
     return run_tile<T, 128, 128, 2, 2>(a, al, s);
 }
 

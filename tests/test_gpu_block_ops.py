@@ -197,6 +197,26 @@ def test_grouped_integers_are_exact(kind):
         assert np.array_equal(y.double().cpu().numpy(), want), (sizes, n, k)
 
 
+@pytest.mark.parametrize("kind", ("f32", "f16", "bf16", "i8"))
+@pytest.mark.parametrize("sizes,n,k", (([1] * 200 + [0, 3], 700, 96), ([20] * 30, 600, 256), ([70, 0, 95, 81], 1100, 200), ([60] * 40, 500, 72),
+                                       ([300, 180, 500], 4000, 64), ([2000, 1777, 0, 2600], 4200, 128), ([2100, 1, 1900, 2500], 4100, 130)), ids=str)
+def test_grouped_every_kernel(sizes, n, k, kind):
+    """Loads on both sides of the launch rules' borders: single rows, a few, dozens and thousands of rows an expert."""
+    okind = "bf16" if kind == "i8" else kind
+    g = sum(sizes) > 6000
+    close(*grouped_run(sizes, n, k, kind, okind, n + k, gather=g, scales=kind == "i8", bias=True, rs=not g, act=1 + g, behind=2, before=3), okind)
+
+
+@pytest.mark.parametrize("kind,okind", (("f32", "f32"), ("f16", "f16"), ("bf16", "f32"), ("i8", "f32"), ("i8", "bf16")))
+@pytest.mark.parametrize("n,k,pads,shift", ((32, 48, (0, 0, 0), 0), (1, 1, (0, 0, 0), 0), (17, 13, (3, 1, 2), 1), (33, 60, (0, 0, 0), 3), (64, 64, (16, 16, 16), 16), (50, 31, (1, 0, 1), 0)))
+def test_grouped_many_short_rows(n, k, pads, shift, kind, okind):
+    """The 1x1 layers of an image network: many rows of few values."""
+    for sizes, act in (([1500, 0, 700, 513], 1), ([2100], 2)):
+        for gather in (False, True):
+            close(*grouped_run(sizes, n, k, kind, okind, n + k, gather=gather, scales=kind == "i8", bias=True, rs=gather, act=act, behind=5, before=1, pads=pads,
+                               shift=shift, bad_src=gather), okind)
+
+
 @pytest.mark.parametrize("kind,okind", (("i8", "bf16"), ("i8", "f16"), ("f32", "bf16"), ("bf16", "f32"), ("f16", "bf16"), ("f16", "f16")))
 @pytest.mark.parametrize("pads,shift", (((0, 0, 0), 1), ((1, 1, 1), 0), ((3, 5, 7), 3), ((16, 16, 16), 16)))
 @pytest.mark.parametrize("load", ("few", "mixed"))
