@@ -55,9 +55,7 @@ struct Tile {
 // The offsets are device memory, so each wave adds up the tiles itself, 64 experts at a time over its lanes.
 template <int TM, int TN>
 struct Tiles {
-    int lo, hi;                // this lane's expert of the first 64, rows [lo, hi)
-    unsigned tiles, sum, all;  // its row tiles, those up to it, those of all experts
-    unsigned nt;               // column tiles
+    unsigned all, nt;  // row tiles of all experts, column tiles
 
     static __device__ __forceinline__ unsigned scan(const qcnn_grouped_matmul_t &a, int e0, int &lo, int &hi, unsigned &tiles)
     {
@@ -79,9 +77,8 @@ struct Tiles {
     __device__ __forceinline__ void count(const qcnn_grouped_matmul_t &a)
     {
         nt = ((unsigned)a.n + TN - 1) / TN;
-        sum = scan(a, 0, lo, hi, tiles);
-        all = __builtin_amdgcn_readlane(sum, 63);
-        for (int e0 = 64; e0 < a.experts; e0 += 64) {
+        all = 0;
+        for (int e0 = 0; e0 < a.experts; e0 += 64) {
             int l, h;
             unsigned n;
             all += __builtin_amdgcn_readlane(scan(a, e0, l, h, n), 63);
@@ -92,8 +89,8 @@ struct Tiles {
     {
         const unsigned per = (all * nt + 7) / 8, at = (blockIdx.x & 7) * per + i;
         if (i >= per || at >= all * nt) return false;
-        int l0 = lo, h0 = hi, e0 = 0;
-        unsigned n = tiles, s = sum, before = 0;
+        int l0, h0, e0 = 0;
+        unsigned n, s = scan(a, 0, l0, h0, n), before = 0;
         for (;;) {
             const unsigned total = __builtin_amdgcn_readlane(s, 63);
             if (at < (before + total) * nt) break;
@@ -268,25 +265,28 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grou
         for (int i = 0; i < LX; ++i) {
             const int r = t.first + min((tid + i * THREADS) >> 2, t.count - 1);
             const int s = a.src ? a.src[r] : r;
-            xp[i] = (const char *)a.x + (size_t)(s >= 0 && s < a.x_rows ? s : 0) * a.ldx * sizeof(T);
+            xp[i] = (const char *)a.x + (size_t)(s >= 0 && s < a.x_rows ? s : 0) * a.ldx * sizeof(T) + (ALIGNED ? chunk : 0);
         }
 #pragma unroll
         for (int i = 0; i < LW; ++i)
-            wp[i] = (const char *)a.w + ((size_t)t.e * a.w_stride + (size_t)min(t.n0 + output_at((tid + i * THREADS) >> 2), a.n - 1) * a.ldw) * sizeof(T);
+            wp[i] = (const char *)a.w + ((size_t)t.e * a.w_stride + (size_t)min(t.n0 + output_at((tid + i * THREADS) >> 2), a.n - 1) * a.ldw) * sizeof(T) +
+                    (ALIGNED ? chunk : 0);
     };
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char *)lds;
     const int steps = (bytes + 63) / 64;
     u32x4 held[ALIGNED ? 1 : LX + LW];
+    // asks for chunk i of the thread's LX + LW of a step; called step after step, the pointers walk
+    const auto request_one = [&](int step, int i, bool ended) {
+        const char *&p = i < LX ? xp[i < LX ? i : 0] : wp[i < LX ? 0 : i - LX];
+        const unsigned at = lds0 + (step & 3) * BUF + wave * 1024 + (i < LX ? i * (THREADS * 16) : TM * 64 + (i - LX) * (THREADS * 16));
+        load_to_lds(ended ? (const char *)&k_zero_chunk : p, at);
+        p += 64;
+    };
     const auto request = [&](int step) {
         if constexpr (ALIGNED) {
-            const int from = step * 64 + chunk;
-            const bool ended = from >= bytes;
-            const unsigned at = lds0 + (step & 3) * BUF + wave * 1024;
+            const bool ended = step * 64 + chunk >= bytes;
 #pragma unroll
-            for (int i = 0; i < LX; ++i) load_to_lds(ended ? (const char *)&k_zero_chunk : xp[i] + (unsigned)from, at + i * (THREADS * 16));
-#pragma unroll
-            for (int i = 0; i < LW; ++i)
-                load_to_lds(ended ? (const char *)&k_zero_chunk : wp[i] + (unsigned)from, at + TM * 64 + i * (THREADS * 16));
+            for (int i = 0; i < LX + LW; ++i) request_one(step, i, ended);
         } else {
 #pragma unroll
             for (int i = 0; i < LX; ++i) held[i] = load_chunk(xp[i], step * 4 + chunk / 16, bytes);
@@ -306,22 +306,23 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grou
 
     const int wm = wave % WM, wn = wave / WM, c16 = lane & 15, g = lane >> 4;
     const int from = c16 * 64 + (g ^ swizzle(c16)) * 16;  // rows of a wave's tiles begin at multiples of 16
-    struct Frags {
-        u32x4 x[FM], w[FN];
-    };
-    const auto read = [&](int step, Frags &f) {
-        const char *bx = lds + (step & 3) * BUF + wm * (TM / WM) * 64 + from, *bw = lds + (step & 3) * BUF + TM * 64 + wn * (TN / WN) * 64 + from;
+    u32x4 fw[FN], fx[2][FM];  // a step's operands; w of the next step takes the place of what has been used
+    const auto read_w = [&](int step, int j) { fw[j] = *(const u32x4 *)(lds + (step & 3) * BUF + from + TM * 64 + wn * (TN / WN) * 64 + j * 1024); };
+    const auto read_x = [&](int step, u32x4(&x)[FM], int i) { x[i] = *(const u32x4 *)(lds + (step & 3) * BUF + from + wm * (TM / WM) * 64 + i * 1024); };
+    const auto read = [&](int step) {
 #pragma unroll
-        for (int i = 0; i < FM; ++i) f.x[i] = *(const u32x4 *)(bx + i * 1024);
+        for (int j = 0; j < FN; ++j) read_w(step, j);
 #pragma unroll
-        for (int j = 0; j < FN; ++j) f.w[j] = *(const u32x4 *)(bw + j * 1024);
+        for (int i = 0; i < FM; ++i) read_x(step, fx[0], i);
     };
     acc_t acc[FN][FM];
-    const auto multiply = [&](const Frags &f) {
+    const auto multiply_part = [&](const u32x4(&x)[FM], int j) {
 #pragma unroll
-        for (int j = 0; j < FN; ++j)
+        for (int i = 0; i < FM; ++i) acc[j][i] = mma(T(), fw[j], x[i], acc[j][i]);
+    };
+    const auto multiply = [&](const u32x4(&x)[FM]) {
 #pragma unroll
-            for (int i = 0; i < FM; ++i) acc[j][i] = mma(T(), f.w[j], f.x[i], acc[j][i]);
+        for (int j = 0; j < FN; ++j) multiply_part(x, j);
     };
     // The chunks of step s have landed, here and (after the barrier) everywhere, and everyone has read step s - 1 into
     // registers.  Loads land in order, so all but those of the two steps behind s are waited for.
@@ -338,7 +339,6 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grou
         }
     };
 
-    Frags f[2];
     const auto begin = [&] {
         request(0);
         if constexpr (ALIGNED) {
@@ -356,28 +356,45 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grou
         if constexpr (ALIGNED) {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (3 < steps) request(3);
-            read(0, f[0]);
-            const auto step = [&](int s, Frags &now, Frags &next) {
+            read(0);
+            // Matrix instructions first: their operands are there.  The reads of the next step and the requests stand between
+            // groups of them, as a wave issues in order and would hold its matrix instructions up behind them: all of them in
+            // front left the matrix cores idle half of the time.  No branch in here; the last steps are made below.
+            const auto step = [&](int s, u32x4(&now)[FM], u32x4(&next)[FM]) {
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * (LX + LW)) : "memory");
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    multiply_part(now, j);
+                    __builtin_amdgcn_sched_barrier(0);
+                    read_w(s + 1, j);
+#pragma unroll
+                    for (int i = FM * j / FN; i < FM * (j + 1) / FN; ++i) read_x(s + 1, next, i);
+#pragma unroll
+                    for (int i = (LX + LW) * j / FN; i < (LX + LW) * (j + 1) / FN; ++i) request_one(s + 4, i, false);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            int s = 0;
+            for (; (s + 6) * 64 <= bytes; s += 2) {
+                step(s, fx[0], fx[1]);
+                step(s + 1, fx[1], fx[0]);
+            }
+#pragma unroll 1
+            for (; s < steps; ++s) {
+                multiply(fx[0]);
                 if (s + 1 < steps) {
                     arrive(s + 1);
                     if (s + 4 < steps) request(s + 4);
-                    read(s + 1, next);
+                    read(s + 1);
                 }
-                multiply(now);
-            };
-            int s = 0;
-            for (; s + 1 < steps; s += 2) {
-                step(s, f[0], f[1]);
-                step(s + 1, f[1], f[0]);
             }
-            if (s < steps) step(s, f[0], f[1]);
         } else {
             for (int s = 0; s < steps; ++s) {
                 deposit(s);
                 arrive(s);
                 if (s + 1 < steps) request(s + 1);
-                read(s, f[0]);
-                multiply(f[0]);
+                read(s);
+                multiply(fx[0]);
             }
         }
         // the next tile's first chunks are on their way while this one's outputs are written
