@@ -21,7 +21,8 @@
 // zero point leave by the sum of x, a product of the same operand with ones:  sum (16 + q) x - (16 + z) sum x.  (Numbers of
 // 16 to 31 where -8 to 7 are meant cost five times the rounding of a float32 sum; exact codes, -8 to 7 by v_cvt_off_f32_i4 or
 // by half arithmetic, took 12 to 14 operations for 8 weights in place of 8 and the time was theirs.)
-// float32 x: three bfloat16 parts (8 + 8 + 8 bits, exact), three instructions.
+// float32 x: three bfloat16 parts (8 + 8 + 8 bits, exact), three instructions.  Its results have the bits to show the rounding
+// of larger sums and its time is that of the parts, so its codes are q - 8, and the sum of x comes in only with zero points.
 #include "block_ops.h"
 
 namespace qcnn {
@@ -82,19 +83,43 @@ __device__ __forceinline__ unsigned and_or(unsigned v, unsigned mask, unsigned m
     return o;
 }
 
-// The 8 codes of a dword as 16 + q, and the ones that go with them
+// (nibble 0 of byte B of v as two's complement) / 16, a float32 whose upper half is the bfloat16
+template <int B>
+__device__ __forceinline__ unsigned sixteenths(unsigned v)
+{
+    unsigned o;
+    if constexpr (B == 0) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(o) : "v"(v));
+    if constexpr (B == 1) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(o) : "v"(v));
+    if constexpr (B == 2) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(o) : "v"(v));
+    if constexpr (B == 3) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(o) : "v"(v));
+    return o;
+}
+
+// The 8 codes of a dword as (q + ADD) / DIV, and the ones that go with them
 template <typename T>
-struct Codes {  // bfloat16, for float32 x too
+struct Codes {  // bfloat16
+    static constexpr float ADD = 16.f, DIV = 1.f;
     static constexpr unsigned BY = 1 << 3 | 1 << 15, MASK = 0x00780078, MAGIC = 0x41804180, ONES = 0x3f803f80;
 };
 template <>
 struct Codes<f16_t> {
+    static constexpr float ADD = 16.f, DIV = 1.f;
     static constexpr unsigned BY = 1 << 6 | 1 << 18, MASK = 0x03c003c0, MAGIC = 0x4c004c00, ONES = 0x3c003c00;
+};
+template <>
+struct Codes<float> {
+    static constexpr float ADD = -8.f, DIV = 16.f;
+    static constexpr unsigned ONES = 0x3f803f80;
 };
 template <typename T>
 __device__ __forceinline__ u32x4 codes(unsigned w)
 {
     typedef Codes<T> C;
+    if constexpr (__is_same(T, float)) {
+        const unsigned even = w ^ 0x88888888u, odd = even >> 4;  // two's complement of q - 8
+        return u32x4{upper_halves(sixteenths<0>(even), sixteenths<0>(odd)), upper_halves(sixteenths<1>(even), sixteenths<1>(odd)),
+                     upper_halves(sixteenths<2>(even), sixteenths<2>(odd)), upper_halves(sixteenths<3>(even), sixteenths<3>(odd))};
+    } else
     return u32x4{and_or(byte_times<0>(w, C::BY), C::MASK, C::MAGIC), and_or(byte_times<1>(w, C::BY), C::MASK, C::MAGIC),
                  and_or(byte_times<2>(w, C::BY), C::MASK, C::MAGIC), and_or(byte_times<3>(w, C::BY), C::MASK, C::MAGIC)};
 }
@@ -310,6 +335,7 @@ __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, un
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[t][m] = f32x4{0, 0, 0, 0};
+    constexpr bool SUM_X = Codes<T>::ADD + 8.f != 0.f || ZERO;
     const bool bf16_scales = a.scale_type == QCNN_BF16;
 
     // a run in registers: everything is asked of LDS before the first of it is used
@@ -359,9 +385,11 @@ __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, un
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     x_operand(T(), r.x[j][m], x[m]);
-                    const u32x4 one = {Codes<T>::ONES, Codes<T>::ONES, Codes<T>::ONES, Codes<T>::ONES};
+                    if (SUM_X) {
+                        const u32x4 one = {Codes<T>::ONES, Codes<T>::ONES, Codes<T>::ONES, Codes<T>::ONES};
 #pragma unroll
-                    for (int p = 0; p < PARTS; ++p) ones[m] = mma(T(), x[m][p], one, ones[m]);
+                        for (int p = 0; p < PARTS; ++p) ones[m] = mma(T(), x[m][p], one, ones[m]);
+                    }
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
@@ -376,11 +404,14 @@ __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, un
             for (int t = 0; t < NT; ++t) {
                 const unsigned u = r.s[f][t];
                 const float s = !S16 ? __uint_as_float(u) : bf16_scales ? __uint_as_float(u << 16) : (float)__builtin_bit_cast(f16_t, (uint16_t)u);
-                const float z = 16.f + (ZERO ? (float)r.z[f][t] : 8.f);
+                const float z = Codes<T>::ADD + (ZERO ? (float)r.z[f][t] : 8.f);
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) acc[t][m][q] = fmaf(s, fmaf(-z, ones[m][q], sum[t][m][q]), acc[t][m][q]);
+                    for (int q = 0; q < 4; ++q) {
+                        const float v = Codes<T>::DIV * sum[t][m][q];
+                        acc[t][m][q] = fmaf(s, SUM_X ? fmaf(-z, ones[m][q], v) : v, acc[t][m][q]);
+                    }
             }
         }
     };
