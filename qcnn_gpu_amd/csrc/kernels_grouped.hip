@@ -5,7 +5,6 @@
 namespace qcnn {
 
 typedef u32x4 u32x4_any __attribute__((aligned(1)));  // global loads and stores take any address
-typedef u32x2 u32x2_any __attribute__((aligned(1)));
 
 // 16 bytes of a row are a chunk; a matrix instruction of 16 x 16 outputs takes a chunk of every lane: lane l holds
 // chunk (l >> 4) of four of row l & 15.  Both operands come in the same order, so the order of k inside a chunk is free:
@@ -113,8 +112,8 @@ struct Tiles {
 // with rows ends in one short tile); workgroups without a tile leave.
 static unsigned most_tiles(const qcnn_grouped_matmul_t &a, int TM) { return (unsigned)(a.rows / TM + (a.experts < a.rows ? a.experts : a.rows)); }
 
-// N neighbouring outputs of one row.  `least` is 0 for ReLU, else -inf (a NaN passes either way).
-template <typename OT, int N>
+// N neighbouring outputs of one row.  `least` is 0 for ReLU, else -inf (a NaN passes either way).  STREAM: past the caches.
+template <typename OT, int N, bool STREAM = false>
 __device__ __forceinline__ void store_row(const qcnn_grouped_matmul_t &a, const float (&v)[N], float rs, float least, size_t r, int n)
 {
     OT o[N];
@@ -122,16 +121,15 @@ __device__ __forceinline__ void store_row(const qcnn_grouped_matmul_t &a, const 
     for (int q = 0; q < N; ++q) from_f32((v[q] < least ? least : v[q]) * rs, o[q]);
     OT *y = (OT *)a.y + r * a.ldy + n;
     if (n + N <= a.n) {
-        if constexpr (sizeof o == 8) {
-            u32x2 c;
-            __builtin_memcpy(&c, o, 8);
-            *(u32x2_any *)y = c;
-        } else {
-            constexpr int C = sizeof o / 16;
-            u32x4 c[C];
-            __builtin_memcpy(c, o, sizeof o);
+        constexpr int C = sizeof o / 16;
+        u32x4 c[C];
+        __builtin_memcpy(c, o, sizeof o);
 #pragma unroll
-            for (int i = 0; i < C; ++i) ((u32x4_any *)y)[i] = c[i];
+        for (int i = 0; i < C; ++i) {
+            if constexpr (STREAM)
+                __builtin_nontemporal_store(c[i], (u32x4_any *)y + i);
+            else
+                ((u32x4_any *)y)[i] = c[i];
         }
     } else {
 #pragma unroll
@@ -614,7 +612,9 @@ static hipError_t run_tile(const qcnn_grouped_matmul_t &a, bool al, hipStream_t 
 // ---- short rows and few outputs, many rows ---------------------------------------------------------------
 // Up to 64 outputs of rows of up to 256 bytes, the 1x1 layers of an image network: reading x and writing y is the cost.
 // A wave keeps the weights of all outputs in registers and runs over its rows, four tiles of sixteen at a time, straight
-// from memory into matrix instructions; four lanes write 64 bytes (float32) of a row side by side.
+// from memory into matrix instructions.  Outputs of two bytes stand in the tiles as output_at has them, so that a lane
+// has 16 bytes of a row either way and four lanes write 64 side by side, past the caches, which the output would only
+// wash out (798720 rows, 48 int8 to 32 float32: 33.6 us, 46.6 through them).
 template <typename T, int NT, int OPS>
 __global__ __launch_bounds__(256) void k_grouped_narrow(const qcnn_grouped_matmul_t a)
 {
@@ -627,16 +627,17 @@ __global__ __launch_bounds__(256) void k_grouped_narrow(const qcnn_grouped_matmu
     if (!tiles.get(a, blockIdx.x >> 3, t)) return;
 
     const int bytes = a.k * (int)sizeof(T);
+    const bool pairs = a.out_type != QCNN_F32;
     u32x4 w[NT][OPS];
     f32x4 ws[NT], b[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        const char *row = (const char *)a.w + ((size_t)t.e * a.w_stride + (size_t)min(j * 16 + c16, a.n - 1) * a.ldw) * sizeof(T);
+        const char *row = (const char *)a.w + ((size_t)t.e * a.w_stride + (size_t)min(pairs ? output_at(j * 16 + c16) : j * 16 + c16, a.n - 1) * a.ldw) * sizeof(T);
 #pragma unroll
         for (int o = 0; o < OPS; ++o) w[j][o] = load_chunk(row, o * 4 + g, bytes);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const size_t n = (size_t)t.e * a.n + min(j * 16 + 4 * g + q, a.n - 1);
+            const size_t n = (size_t)t.e * a.n + min((pairs ? output_at(j * 16 + 4 * g) : j * 16 + 4 * g) + q, a.n - 1);
             ws[j][q] = a.w_scale ? a.w_scale[n] : 1.f;
             b[j][q] = a.bias ? a.bias[n] : 0.f;
         }
@@ -661,19 +662,24 @@ __global__ __launch_bounds__(256) void k_grouped_narrow(const qcnn_grouped_matmu
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
                 const int m = m0 + i * 16 + c16;
+                constexpr int N = 16 / sizeof(OT), TILES = N / 4;  // outputs side by side, of so many tiles
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    acc_t acc = {0, 0, 0, 0};
+                for (int j = 0; j < NT; j += TILES) {
+                    float v[N];
 #pragma unroll
-                    for (int o = 0; o < OPS; ++o) acc = mma(T(), w[j][o], x[i][o], acc);
-                    float v[4];
+                    for (int h = 0; h < TILES; ++h) {
+                        acc_t acc = {0, 0, 0, 0};
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) v[q] = (have[i] ? (float)acc[q] * ws[j][q] * xs[i] : 0.f) + b[j][q];
+                        for (int o = 0; o < OPS; ++o) acc = mma(T(), w[j + h][o], x[i][o], acc);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) v[4 * h + q] = (have[i] ? (float)acc[q] * ws[j + h][q] * xs[i] : 0.f) + b[j + h][q];
+                    }
                     if (a.act == QCNN_ACT_SILU) {
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) v[q] = block_act(v[q], QCNN_ACT_SILU);
+                        for (int q = 0; q < N; ++q) v[q] = block_act(v[q], QCNN_ACT_SILU);
                     }
-                    if (m < t.count && j * 16 + 4 * g < a.n) store_row<OT>(a, v, rs[i], least, (size_t)(t.first + m), j * 16 + 4 * g);
+                    const int n = j * 16 + N * g;
+                    if (m < t.count && n < a.n) store_row<OT, N, true>(a, v, rs[i], least, (size_t)(t.first + m), n);
                 }
             }
         }
@@ -707,6 +713,7 @@ static hipError_t pick(qcnn_grouped_matmul_t a, hipStream_t s)
     const auto tiles = [&](long long tm, long long tn) { return (a.rows / tm + groups) * ((a.n + tn - 1) / tn); };
     if (a.n <= 64 && a.k * z <= 256 && avg >= 512) {
         if (a.k * z <= 64) return a.n <= 32 ? run_narrow<T, 2, 1>(a, s) : run_narrow<T, 4, 1>(a, s);
+        if (a.k * z <= 128) return a.n <= 32 ? run_narrow<T, 2, 2>(a, s) : run_narrow<T, 4, 2>(a, s);
         return a.n <= 32 ? run_narrow<T, 2, 4>(a, s) : run_narrow<T, 4, 4>(a, s);
     }
     if (avg <= 4) return tiles(16, 32) < 256 ? run_rows<T, 1, 128, 8, 1, 80>(a, al, s) : run_rows<T, 1, 128, 4, 2, 80>(a, al, s);
