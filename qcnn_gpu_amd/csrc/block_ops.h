@@ -61,6 +61,13 @@ __device__ __forceinline__ float block_act(float v, int act)
 
 hipError_t launch_matvec_w4(const qcnn_matvec_w4_t &a, hipStream_t s);
 hipError_t launch_grouped_matmul(const qcnn_grouped_matmul_t &a, hipStream_t s);
-hipError_t launch_norm_res(const qcnn_norm_res_t &a, hipStream_t s);
+template <typename T>
+hipError_t norm_res_of(const qcnn_norm_res_t &a, hipStream_t s);
+inline hipError_t launch_norm_res(const qcnn_norm_res_t &a, hipStream_t s)
+{
+    if (a.type == QCNN_F32) return norm_res_of<float>(a, s);
+    if (a.type == QCNN_F16) return norm_res_of<f16_t>(a, s);
+    return norm_res_of<bf16_t>(a, s);
+}
 
 }  // namespace qcnn

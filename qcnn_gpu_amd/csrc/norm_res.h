@@ -1,4 +1,4 @@
-// The two ends of a residual block (qcnn_op_norm_res): post norm, gate, scaled residual addition and the next
+// The two ends of a residual block (qcnn_op_norm_res; kernels_norm_*.hip make a type of it each): post norm, gate, scaled residual addition and the next
 // block's norm in one pass over the row.
 //
 //   s = sum_j y[index[r][j]];  h = beta x + alpha act(gate) post(s);  n = pre(h)
@@ -8,6 +8,7 @@
 // chunk c of a row belonging to thread c mod LPR, so that neighbouring threads touch neighbouring addresses.
 // Loads and stores take any alignment; only the chunk that the end of a row cuts goes by elements.
 // Statistics are float32 (the variance as the mean of the squared distances from the mean, from the registers).
+#pragma once
 #include "block_ops.h"
 
 namespace qcnn {
@@ -35,10 +36,14 @@ struct Chunk {
             __builtin_memcpy(&raw, t, 16);
         }
     }
+    template <bool STREAM>
     __device__ __forceinline__ void store(T *p, int left) const
     {
         if (left >= VE) {
-            *(u32x4_any *)p = raw;
+            if constexpr (STREAM)
+                __builtin_nontemporal_store(raw, (u32x4_any *)p);
+            else
+                *(u32x4_any *)p = raw;
         } else {
             T t[VE];
             __builtin_memcpy(t, &raw, 16);
@@ -122,7 +127,7 @@ __device__ __forceinline__ float tanh_of(float u)
     return fabsf(u) < 0.3f ? u * p : e;
 }
 
-template <typename T, int LPR, int CPT>
+template <typename T, int LPR, int CPT, bool STREAM>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void k_norm_res(const qcnn_norm_res_t a)
 {
     typedef Chunk<T> C;
@@ -224,13 +229,15 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void k_norm_res(const qcnn_n
         if (g) {
             if (!EARLY) gr[0].load(g + at, d - at);
             gr[EARLY ? c : 0].get(u);
+            if (a.act == QCNN_GATE_TANH) {
 #pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                if (a.act == QCNN_GATE_SIGMOID) u[i] = sigmoid(u[i]);
-                if (a.act == QCNN_GATE_TANH) u[i] = tanh_of(u[i]);
-                if (a.act == QCNN_GATE_SILU) u[i] = u[i] * sigmoid(u[i]);
-                v[c][i] *= u[i];
+                for (int i = 0; i < VE; ++i) u[i] = tanh_of(u[i]);
+            } else if (a.act != QCNN_GATE_LINEAR) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) u[i] = (a.act == QCNN_GATE_SILU ? u[i] : 1.f) * sigmoid(u[i]);
             }
+#pragma unroll
+            for (int i = 0; i < VE; ++i) v[c][i] *= u[i];
         }
         if (!EARLY) xr[0].load(x + at, d - at);
         xr[EARLY ? c : 0].get(u);
@@ -239,7 +246,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void k_norm_res(const qcnn_n
         if (a.h) {
             C o;
             o.set(v[c]);
-            o.store((T *)a.h + r * a.ldh + at, d - at);
+            o.template store<STREAM>((T *)a.h + r * a.ldh + at, d - at);
         }
     }
     if (!a.n) return;
@@ -250,7 +257,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void k_norm_res(const qcnn_n
         if (at >= d) continue;
         C o;
         o.set(v[c]);
-        o.store((T *)a.n + r * a.ldn + at, d - at);
+        o.template store<STREAM>((T *)a.n + r * a.ldn + at, d - at);
     }
 }
 
@@ -258,34 +265,38 @@ template <typename T, int LPR, int CPT>
 static hipError_t run(const qcnn_norm_res_t &a, hipStream_t s)
 {
     constexpr int BLOCK = LPR > 256 ? LPR : 256, RPB = BLOCK / LPR;
-    k_norm_res<T, LPR, CPT><<<(unsigned)((a.rows + RPB - 1) / RPB), BLOCK, 0, s>>>(a);
+    // Outputs from 8 MB on are written past the caches: 2048 x 8192 bf16 36.4 -> 28.8 us, 16384 x 4096 156 -> 152.  A reader right behind
+    // takes as long either way (4096 x 1024 and two readers 18.8 -> 17.8, 16384 x 4096 207 -> 206), but finds smaller ones sooner in
+    // the caches (256 x 4096 and two readers 11.6, 12.0 past them).
+    const bool stream = (size_t)a.rows * a.d * sizeof(T) * ((a.h != nullptr) + (a.n != nullptr)) >= (size_t)8 << 20;
+    const unsigned blocks = (unsigned)((a.rows + RPB - 1) / RPB);
+    if (stream)
+        k_norm_res<T, LPR, CPT, true><<<blocks, BLOCK, 0, s>>>(a);
+    else
+        k_norm_res<T, LPR, CPT, false><<<blocks, BLOCK, 0, s>>>(a);
     return hipGetLastError();
 }
 
-// Threads a row and chunks a thread: a row of at most 128 chunks fits one wave (no barrier).
+// Threads a row and chunks a thread.  A row of at most 64 chunks fits one wave (no barrier).  With up to 512 rows the time is one
+// row's latency: a chunk a thread (1 x 4096 bf16 5.2 -> 3.9 us, 256 x 8192 10.1 -> 6.7); with more, two and four chunks a thread keep
+// more rows on a CU (16384 x 4096: 156 us, 170 with one; 2048 x 8192: 36.4, 42.6 with one).
 template <typename T>
-static hipError_t pick(const qcnn_norm_res_t &a, hipStream_t s)
+hipError_t norm_res_of(const qcnn_norm_res_t &a, hipStream_t s)
 {
     const int c = (a.d + Chunk<T>::VE - 1) / Chunk<T>::VE;
+    const bool few = a.rows <= 512;
     if (c <= 8) return run<T, 8, 1>(a, s);
     if (c <= 16) return run<T, 16, 1>(a, s);
     if (c <= 32) return run<T, 32, 1>(a, s);
     if (c <= 64) return run<T, 64, 1>(a, s);
-    if (c <= 128) return run<T, 64, 2>(a, s);
+    if (c <= 128 && !few) return run<T, 64, 2>(a, s);
     if (c <= 256) return run<T, 256, 1>(a, s);
-    if (c <= 512) return run<T, 256, 2>(a, s);
-    if (c <= 1024) return run<T, 256, 4>(a, s);
+    if (c <= 512) return few ? run<T, 512, 1>(a, s) : run<T, 256, 2>(a, s);
+    if (c <= 1024) return few ? run<T, 1024, 1>(a, s) : run<T, 256, 4>(a, s);
     if (c <= 2048) return run<T, 1024, 2>(a, s);
     if (c <= 4096) return run<T, 1024, 4>(a, s);
     if (c <= 8192) return run<T, 1024, 8>(a, s);
     return run<T, 1024, 16>(a, s);  // float32 rows of up to 65536
-}
-
-hipError_t launch_norm_res(const qcnn_norm_res_t &a, hipStream_t s)
-{
-    if (a.type == QCNN_F32) return pick<float>(a, s);
-    if (a.type == QCNN_F16) return pick<f16_t>(a, s);
-    return pick<bf16_t>(a, s);
 }
 
 }  // namespace qcnn

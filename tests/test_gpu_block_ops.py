@@ -285,9 +285,10 @@ def test_norm_row_lengths(d, kind):
 
 
 @pytest.mark.parametrize("kind", ("f32", "bf16"))
-@pytest.mark.parametrize("rows", (1, 2, 31, 32, 33, 1000))
+@pytest.mark.parametrize("rows", (1, 2, 31, 32, 33, 512, 513, 1000))
 def test_norm_row_counts(rows, kind):
-    for d in (40, 130, 600):
+    """512 rows, and with them outputs of 8 MB, are borders of the launch rules."""
+    for d in (40, 130, 600, 1025, 3000, 6001):
         norm_run(rows, d, kind, "f32", 2, 1, rows + d, gate=3, act=1, parts=2)
 
 
