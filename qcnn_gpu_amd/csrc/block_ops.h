@@ -3,6 +3,8 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
+#include <atomic>
+
 #include "qcnn_internal.h"
 
 namespace qcnn {
@@ -57,6 +59,21 @@ __device__ __forceinline__ float block_act(float v, int act)
     if (act == QCNN_ACT_RELU) return v < 0.f ? 0.f : v;
     if (act == QCNN_ACT_SILU) return v / (1.f + __expf(-v));
     return v;
+}
+
+// Lets kernel `fn` have `bytes` of LDS beyond the 64 KB that need no asking; `asked` holds a bit for each device on which that has
+// been done (asking again at every launch is 0.5 us of the caller's time).
+inline hipError_t allow_lds(const void *fn, int bytes, std::atomic<unsigned long long> &asked)
+{
+    if (bytes <= 65536) return hipSuccess;
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (asked.load(std::memory_order_relaxed) & bit)) return hipSuccess;
+    e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess && dev < 64) asked.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 hipError_t launch_matvec_w4(const qcnn_matvec_w4_t &a, hipStream_t s);

@@ -234,7 +234,7 @@ __device__ __forceinline__ void load_to_lds(const char *from, unsigned lds)
 // ds_read_b128 serves at a time (rows 0-3 and 12-15 of one chunk, 4-11 of the next) then touch sixteen different slots
 // of the 256 bytes that the banks hold.
 // ALIGNED (rows begin at multiples of 16 bytes and hold whole chunks): loads go straight to LDS, a lane whose row
-// has ended loads zeros.  Otherwise loads of any address go through registers, one step ahead.
+// has ended loads zeros.  Otherwise loads of any address go through registers, a step ahead of LDS.
 template <typename T, int TM, int TN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grouped_matmul_t a)
 {
@@ -322,19 +322,15 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grou
 #pragma unroll
         for (int j = 0; j < FN; ++j) multiply_part(x, j);
     };
-    // The chunks of step s have landed, here and (after the barrier) everywhere, and everyone has read step s - 1 into
-    // registers.  Loads land in order, so all but those of the two steps behind s are waited for.
+    // (ALIGNED) The chunks of step s have landed, here and (after the barrier) everywhere, and everyone has read step s - 1
+    // into registers.  Loads land in order, so all but those of the two steps behind s are waited for.
     const auto arrive = [&](int s) {
-        if constexpr (ALIGNED) {
-            if (s + 2 < steps)
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * (LX + LW)) : "memory");
-            else if (s + 1 < steps)
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LX + LW) : "memory");
-            else
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        } else {
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        }
+        if (s + 2 < steps)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * (LX + LW)) : "memory");
+        else if (s + 1 < steps)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LX + LW) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
 
     const auto begin = [&] {
@@ -387,12 +383,21 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grou
                 }
             }
         } else {
+            // Step s: s + 1 is in LDS, s + 2 is put there and s + 3 asked for, behind the matrix instructions of s.
+            deposit(0);
+            if (1 < steps) request(1);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            read(0);
+            if (1 < steps) deposit(1);
+            if (2 < steps) request(2);
+#pragma unroll 1
             for (int s = 0; s < steps; ++s) {
-                deposit(s);
-                arrive(s);
-                if (s + 1 < steps) request(s + 1);
-                read(s);
+                if (s + 1 < steps) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 multiply(fx[0]);
+                __builtin_amdgcn_sched_barrier(0);
+                if (s + 1 < steps) read(s + 1);
+                if (s + 2 < steps) deposit(s + 2);
+                if (s + 3 < steps) request(s + 3);
             }
         }
         // the next tile's first chunks are on their way while this one's outputs are written
@@ -472,7 +477,8 @@ __global__ __launch_bounds__(64 * KW *NW) void k_grouped_rows(const qcnn_grouped
     char *const ring = lds + kq * (R * G::RUN);
     const unsigned ring_at = (unsigned)(size_t)(__attribute__((address_space(3))) char *)ring;
     int bring_slot = 0;
-    // brings run i (of this group) into the ring; called for 0, 1, 2 ...
+    u32x4 held[ALIGNED ? 1 : OPS + G::XL];
+    // brings run i (of this group) into the ring, or (not ALIGNED) into registers; called for 0, 1, 2 ...
     const auto bring = [&](int i) {
         if (i < count) {
             const int left = bytes - (first + i) * RB - g * 16;  // bytes of the rows from this lane's first chunk on
@@ -486,22 +492,28 @@ __global__ __launch_bounds__(64 * KW *NW) void k_grouped_rows(const qcnn_grouped
                     if (has[j]) load_to_lds(o * 64 < left ? xp[j] + o * 64 : (const char *)&k_zero_chunk, at + (j * NW + nq) * 1024);
                 }
             } else {
-                char *at = ring + bring_slot + lane * 16;
-                u32x4 v[OPS + G::XL];
 #pragma unroll
-                for (int o = 0; o < OPS; ++o) v[o] = load_chunk(wp, o * 4, left);
+                for (int o = 0; o < OPS; ++o) held[o] = load_chunk(wp, o * 4, left);
 #pragma unroll
-                for (int j = 0; j < G::XL; ++j) v[OPS + j] = load_chunk(xp[j], (j * NW + nq) % OPS * 4, left);
-#pragma unroll
-                for (int o = 0; o < OPS; ++o) *(u32x4 *)(at + G::XB + (nq * OPS + o) * 1024) = v[o];
-#pragma unroll
-                for (int j = 0; j < G::XL; ++j) *(u32x4 *)(at + (j * NW + nq) * 1024) = v[OPS + j];
+                for (int j = 0; j < G::XL; ++j) held[OPS + j] = load_chunk(xp[j], (j * NW + nq) % OPS * 4, left);
             }
             wp += RB;
 #pragma unroll
             for (int j = 0; j < G::XL; ++j) xp[j] += RB;
         }
-        bring_slot = bring_slot == (R - 1) * G::RUN ? 0 : bring_slot + G::RUN;
+        if constexpr (ALIGNED) bring_slot = bring_slot == (R - 1) * G::RUN ? 0 : bring_slot + G::RUN;
+    };
+    const auto deposit = [&](int i) {  // run i, from registers
+        if constexpr (!ALIGNED) {
+            if (i < count) {
+                char *at = ring + bring_slot + lane * 16;
+#pragma unroll
+                for (int o = 0; o < OPS; ++o) *(u32x4 *)(at + G::XB + (nq * OPS + o) * 1024) = held[o];
+#pragma unroll
+                for (int j = 0; j < G::XL; ++j) *(u32x4 *)(at + (j * NW + nq) * 1024) = held[OPS + j];
+            }
+            bring_slot = bring_slot == (R - 1) * G::RUN ? 0 : bring_slot + G::RUN;
+        }
     };
     wp += g * 16;
 #pragma unroll
@@ -511,14 +523,28 @@ __global__ __launch_bounds__(64 * KW *NW) void k_grouped_rows(const qcnn_grouped
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[m] = acc_t{0, 0, 0, 0};
     int slot = 0;
+    if constexpr (ALIGNED) {
 #pragma unroll 1
-    for (int i = 0; i < R - 1; ++i) bring(i);
+        for (int i = 0; i < R - 1; ++i) bring(i);
+    } else {
+        bring(0);
+        deposit(0);
+        bring(1);
+    }
     for (int i = 0; i < turns; ++i) {
         // run i has landed (loads land in order: all but those of the runs behind it), here and after the barrier for all, and
-        // everyone is done with run i - 1, whose place run i + R - 1 takes
-        wait_for_all_but<R - 2, G::LOADS>(count - 1 - i);
+        // everyone is done with run i - 1, whose place run i + R - 1 takes (not ALIGNED: run i + 1, from registers; R >= 2)
+        if constexpr (ALIGNED)
+            wait_for_all_but<R - 2, G::LOADS>(count - 1 - i);
+        else
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (NW > 1) asm volatile("s_barrier" ::: "memory");
-        bring(i + R - 1);
+        if constexpr (ALIGNED) {
+            bring(i + R - 1);
+        } else {
+            deposit(i + 1);
+            bring(i + 2);
+        }
         if (i < count) {
             const char *at = ring + slot + lane * 16;
             u32x4 w[OPS], x[OPS][MT];
@@ -570,11 +596,10 @@ static hipError_t run_rows(const qcnn_grouped_matmul_t &a, bool al, hipStream_t 
     const unsigned long long tiles = (unsigned long long)most_tiles(a, 16 * MT) * ((a.n + 16 * NW - 1) / (16 * NW));
     const unsigned long long blocks = (tiles + 7) / 8 * 8;  // as many on each XCD
     if (blocks * (64 * KW * NW) > 0xffffffffull) return hipErrorInvalidConfiguration;
+    static std::atomic<unsigned long long> asked[2] = {{0}, {0}};
     const auto fn = al ? k_grouped_rows<T, MT, RB, KW, NW, KB, true> : k_grouped_rows<T, MT, RB, KW, NW, KB, false>;
-    if (G::LDS > 65536) {
-        const hipError_t e = hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
-        if (e != hipSuccess) return e;
-    }
+    const hipError_t e = allow_lds((const void *)fn, G::LDS, asked[al]);
+    if (e != hipSuccess) return e;
     fn<<<(unsigned)blocks, 64 * KW * NW, G::LDS, s>>>(a);
     return hipGetLastError();
 }
@@ -597,15 +622,14 @@ static hipError_t run_tile(const qcnn_grouped_matmul_t &a, bool al, hipStream_t 
     const unsigned long long tiles = (unsigned long long)most_tiles(a, TM) * ((a.n + TN - 1) / TN);
     const unsigned long long fit = (unsigned long long)compute_units() * PER_CU;
     const unsigned blocks = (unsigned)(((tiles < fit ? tiles : fit) + 7) / 8 * 8);  // as many on each XCD; they walk the tiles
-    const void *fn = al ? (const void *)k_grouped_tile<T, TM, TN, WM, WN, true> : (const void *)k_grouped_tile<T, TM, TN, WM, WN, false>;
-    if (LDS > 65536) {
-        const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-        if (e != hipSuccess) return e;
+    auto fn = k_grouped_tile<T, TM, TN, WM, WN, true>;
+    if constexpr (TM < 256) {  // (the largest tiles have no registers for loads of any address)
+        if (!al) fn = k_grouped_tile<T, TM, TN, WM, WN, false>;
     }
-    if (al)
-        k_grouped_tile<T, TM, TN, WM, WN, true><<<blocks, 64 * WM * WN, LDS, s>>>(a);
-    else
-        k_grouped_tile<T, TM, TN, WM, WN, false><<<blocks, 64 * WM * WN, LDS, s>>>(a);
+    static std::atomic<unsigned long long> asked[2] = {{0}, {0}};
+    const hipError_t e = allow_lds((const void *)fn, LDS, asked[al]);
+    if (e != hipSuccess) return e;
+    fn<<<blocks, 64 * WM * WN, LDS, s>>>(a);
     return hipGetLastError();
 }
 
@@ -615,11 +639,11 @@ static hipError_t run_tile(const qcnn_grouped_matmul_t &a, bool al, hipStream_t 
 // from memory into matrix instructions.  Outputs of two bytes stand in the tiles as output_at has them, so that a lane
 // has 16 bytes of a row either way and four lanes write 64 side by side, past the caches, which the output would only
 // wash out (798720 rows, 48 int8 to 32 float32: 33.6 us, 46.6 through them).
-template <typename T, int NT, int OPS>
+template <typename T, int NT, int OPS, int TM>
 __global__ __launch_bounds__(256) void k_grouped_narrow(const qcnn_grouped_matmul_t a)
 {
     typedef typename Mma<T>::acc_t acc_t;
-    constexpr int TM = 512, BATCH = OPS == 1 ? 4 : 2;  // rows of a workgroup; row tiles on their way at a time
+    constexpr int BATCH = TM == 64 ? 1 : OPS == 1 ? 4 : 2;  // row tiles on their way at a time
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
     Tiles<TM, 64> tiles;
     tiles.count(a);
@@ -692,13 +716,20 @@ __global__ __launch_bounds__(256) void k_grouped_narrow(const qcnn_grouped_matmu
         rows(bf16_t());
 }
 
+template <typename T, int NT, int OPS, int TM>
+static hipError_t launch_narrow(const qcnn_grouped_matmul_t &a, hipStream_t s)
+{
+    const unsigned long long blocks = ((unsigned long long)most_tiles(a, TM) + 7) / 8 * 8;
+    if (blocks * 256 > 0xffffffffull) return hipErrorInvalidConfiguration;
+    k_grouped_narrow<T, NT, OPS, TM><<<(unsigned)blocks, 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+// 512 rows a workgroup where that makes enough of them, else 64 (3968 rows of 209 bytes 28 -> 9 us).
 template <typename T, int NT, int OPS>
 static hipError_t run_narrow(const qcnn_grouped_matmul_t &a, hipStream_t s)
 {
-    const unsigned long long blocks = ((unsigned long long)most_tiles(a, 512) + 7) / 8 * 8;
-    if (blocks * 256 > 0xffffffffull) return hipErrorInvalidConfiguration;
-    k_grouped_narrow<T, NT, OPS><<<(unsigned)blocks, 256, 0, s>>>(a);
-    return hipGetLastError();
+    return a.rows >= 131072 ? launch_narrow<T, NT, OPS, 512>(a, s) : launch_narrow<T, NT, OPS, 64>(a, s);
 }
 
 template <typename T>
@@ -709,6 +740,14 @@ static hipError_t pick(qcnn_grouped_matmul_t a, hipStream_t s)
     const bool al = (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.w % 16 == 0 && a.ldx * z % 16 == 0 && a.ldw * z % 16 == 0 && a.w_stride * z % 16 == 0 &&
                     a.k * z % 16 == 0;
     // Which kernel, by the rows an expert has on average (the host does not know the offsets) and the tiles there can be.
+    // Microseconds of the taken side and of the other, skewed loads, cold memory:
+    //   narrow    798720 rows 48 -> 32 int8            33, tiles 136
+    //   rows      64 over 64 experts, 1024 x 2048      34, 128 x 128 tiles 53;  7 rows 157 x 3840: 8 k groups 8.5, 4 26
+    //             128 over 16, 2048 x 2048             30, 16 rows a workgroup 36;  200 over 8, 300 x 1000: 7.5, 64 x 64 tiles 8.8
+    //   64 x 64   1024 over 16, 1024 x 1024            13, 128 x 128 20;  512 over 4, 1024 x 1024: 9.5, rows 20;
+    //             float32 5000 over 5, 1000 x 2000    201, 128 x 128 254
+    //   128 x 128 8900 over 22, 1424 x 1944           134, 256 x 256 167;  8192 over 64, 2048 x 2048: 176, 256 x 256 216
+    //   256 x 256 16384 over 16, 4096 x 2048          337, 128 x 128 403;  int8 6000 over 8, 2048 x 2048: 39, 128 x 128 47
     const long long groups = a.rows < a.experts ? a.rows : a.experts, avg = a.rows / a.experts;
     const auto tiles = [&](long long tm, long long tn) { return (a.rows / tm + groups) * ((a.n + tn - 1) / tn); };
     if (a.n <= 64 && a.k * z <= 256 && avg >= 512) {
@@ -716,11 +755,15 @@ static hipError_t pick(qcnn_grouped_matmul_t a, hipStream_t s)
         if (a.k * z <= 128) return a.n <= 32 ? run_narrow<T, 2, 2>(a, s) : run_narrow<T, 4, 2>(a, s);
         return a.n <= 32 ? run_narrow<T, 2, 4>(a, s) : run_narrow<T, 4, 4>(a, s);
     }
-    if (avg <= 4) return tiles(16, 32) < 256 ? run_rows<T, 1, 128, 8, 1, 80>(a, al, s) : run_rows<T, 1, 128, 4, 2, 80>(a, al, s);
-    if (tiles(64, 64) < 256) return run_rows<T, 2, 128, 4, 2, 80>(a, al, s);
+    if (tiles(32, 32) < 128) return run_rows<T, 1, 256, 8, 1, 160>(a, al, s);
+    if (avg <= 24 && a.k * z <= 512) return run_rows<T, 1, 256, 1, 4, 40>(a, al, s);  // nothing to split k for: 61 rows over 82, 2334 x 71 int8: 11 us, split 31
+    if (avg <= 4) return run_rows<T, 1, 128, 4, 2, 80>(a, al, s);
+    if (tiles(64, 64) < 64) return run_rows<T, 2, 128, 4, 2, 80>(a, al, s);
     if (avg <= 24) return run_rows<T, 4, 128, 2, 4, 80>(a, al, s);
-    if (tiles(128, 128) < 256) return run_tile<T, 64, 64, 2, 2>(a, al, s);
-    if (sizeof(T) < 4 && al && tiles(256, 256) >= 512) return run_tile<T, 256, 256, 2, 4>(a, al, s);
+    if (tiles(128, 128) < (sizeof(T) == 4 ? 1024 : 256)) return run_tile<T, 64, 64, 2, 2>(a, al, s);
+    if constexpr (sizeof(T) < 4) {
+        if (al && avg >= 256 && tiles(256, 256) >= (sizeof(T) == 1 ? 240 : 512)) return run_tile<T, 256, 256, 2, 4>(a, al, s);
+    }
     return run_tile<T, 128, 128, 2, 2>(a, al, s);
 }
 

@@ -462,10 +462,9 @@ static hipError_t launch(const qcnn_matvec_w4_t &a, hipStream_t s)
     const unsigned long long blocks = (unsigned long long)nblocks * ((a.rows + XROWS - 1) / XROWS);
     if (blocks * (64 * G::WAVES) > 0xffffffffull) return hipErrorInvalidConfiguration;
     const auto fn = k_w4<T, NT, XROWS, FL, S16, ZERO, KW, NW, KB>;
-    if (G::LDS > 65536) {
-        const hipError_t e = hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
-        if (e != hipSuccess) return e;
-    }
+    static std::atomic<unsigned long long> asked{0};
+    const hipError_t e = allow_lds((const void *)fn, G::LDS, asked);
+    if (e != hipSuccess) return e;
     fn<<<(unsigned)blocks, 64 * G::WAVES, G::LDS, s>>>(a, nblocks);
     return hipGetLastError();
 }
@@ -484,21 +483,32 @@ static hipError_t run(const qcnn_matvec_w4_t &a, hipStream_t s)
 // 16384, the taken side of each border first:
 //   bfloat16 rows <= 4     4.6 / 4.9 / 7.2 / 11.0   (KB 80: 4.7 / 5.4 / 7.6 / 12.9;  two tiles a wave 6.1 / 6.3 / 7.4 / 10.8)
 //            rows <= 16    8 x 1 5.5 / 6.4 / 12.0 / 21.9 up to 4096, 4 x 2 7.6 / 8.1 / 9.1 / 14.2 above
-//            rows <= 64    32 rows 4 x 2 9.5 / 11.0 / 20.4 / 40.1 up to 4096, 64 rows 2 x 4 20.5 / 22.4 / 23.0 / 26.8 above
+//            64 rows       32 rows 4 x 2 9.5 / 11.0 / 20.4 / 40.1 up to 4096, 4 x 4 12.9 / 14.4 / 15.7 / 31.3 up to 8192 (and up
+//                          to 32 rows), 64 rows 2 x 4 20.5 / 22.4 / 23.0 / 26.8 above
 //   float32  rows <= 4     one tile 7.4 / 8.1 / 13.5 / 22.9 up to 4096, two 8.6 / 9.2 / 10.2 / 16.9 above
 //            rows <= 16    one tile 13.1 / 14.1 / 15.5 / 30.1 up to 8192, two 17.2 / 18.5 / 19.5 / 21.8 above
-//            rows <= 64    16 rows 4 x 4 20.5 / 24.1 / 44.4 / 96.1 up to 4096, 32 rows, two tiles 47.2 / 49.4 / 49.7 / 60.1 above
+//            64 rows       16 rows 4 x 4 20.5 / 24.1 / 44.4 / 96.1 up to 8192 (and up to 32 rows), 32 rows, two tiles 47.2 / 49.4 /
+//                          49.7 / 60.1 above
+// Where that leaves fewer than 128 workgroups, sixteen rows and sixteen outputs each with the most waves along k that fit:
+// 9 x 167 x 12134 float32 56 -> 25 us, 22 x 128 x 10048 bfloat16 25 -> 11.
 template <typename T, int FL>
 static hipError_t pick_rows(const qcnn_matvec_w4_t &a, hipStream_t s)
 {
-    if constexpr (sizeof(T) == 4) {
-        if (a.rows <= 4) return a.n <= 4096 ? run<T, 1, 4, FL, 8, 1, 80>(a, s) : run<T, 2, 4, FL, 8, 1, 80>(a, s);
+    constexpr bool F = sizeof(T) == 4;
+    const auto groups = [&](long long rows, long long outputs) { return ((a.rows + rows - 1) / rows) * ((a.n + outputs - 1) / outputs); };
+    if (a.rows <= 4) {
+        if (groups(4, 16) < 128) return run<T, 1, 4, FL, 16, 1, F ? 160 : 106>(a, s);
+        if constexpr (F) return a.n <= 4096 ? run<T, 1, 4, FL, 8, 1, 80>(a, s) : run<T, 2, 4, FL, 8, 1, 80>(a, s);
+        return run<T, 1, 4, FL, 8, 1, 53>(a, s);
+    }
+    if (groups(32, 32) < 128) return run<T, 1, 16, FL, 8, 1, 160>(a, s);
+    if constexpr (F) {
         if (a.rows <= 16) return a.n <= 8192 ? run<T, 1, 16, FL, 4, 2, 80>(a, s) : run<T, 2, 16, FL, 4, 2, 160>(a, s);
-        return a.n <= 4096 ? run<T, 1, 16, FL, 4, 4, 160>(a, s) : run<T, 2, 32, FL, 2, 4, 160>(a, s);
+        return a.rows <= 32 || a.n <= 8192 ? run<T, 1, 16, FL, 4, 4, 160>(a, s) : run<T, 2, 32, FL, 2, 4, 160>(a, s);
     } else {
-        if (a.rows <= 4) return run<T, 1, 4, FL, 8, 1, 53>(a, s);
         if (a.rows <= 16) return a.n <= 4096 ? run<T, 1, 16, FL, 8, 1, 160>(a, s) : run<T, 1, 16, FL, 4, 2, 80>(a, s);
-        return a.n <= 4096 ? run<T, 1, 32, FL, 4, 2, 160>(a, s) : run<T, 1, 64, FL, 2, 4, 160>(a, s);
+        if (a.n <= 4096) return run<T, 1, 32, FL, 4, 2, 160>(a, s);
+        return a.rows <= 32 || a.n <= 8192 ? run<T, 1, 32, FL, 4, 4, 160>(a, s) : run<T, 1, 64, FL, 2, 4, 160>(a, s);
     }
 }
 

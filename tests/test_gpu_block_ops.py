@@ -99,8 +99,8 @@ def test_w4_against_the_definition(shape, zeros, kind):
 
 
 @pytest.mark.parametrize("kind", ("f32", "f16", "bf16"))
-@pytest.mark.parametrize("rows", (1, 4, 5, 16, 17, 64, 70))
-@pytest.mark.parametrize("n,k,group", ((4096, 384, 64), (4100, 256, 32), (8200, 300, 128), (4097, 1000, 96)))
+@pytest.mark.parametrize("rows", (1, 4, 5, 16, 17, 33, 64, 70))
+@pytest.mark.parametrize("n,k,group", ((4096, 384, 64), (4100, 256, 32), (8200, 300, 128), (4097, 1000, 96), (150, 5000, 64)))
 def test_w4_many_outputs(n, k, group, rows, kind):
     """Both sides of every border of the launch rules, groups of all three kinds, a last workgroup that is not full."""
     d = w4_data(rows, n, k, group, kind, True, True, n + rows)
