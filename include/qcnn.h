@@ -385,7 +385,8 @@ enum { QCNN_ACT_NONE = 0, QCNN_ACT_RELU = 1, QCNN_ACT_SILU = 2 };
 /* Products grouped by expert: rows offsets[e] .. offsets[e+1] - 1 of y belong to weight set e,
  *   y[r][j] = row_scale[r] * act(w_scale[e][j] * x_scale[s] * sum_k w[e][j][k] * x[s][k]  + bias[e][j]),  s = src[r]
  * The offsets are read on the device; the call's shape depends on `rows` alone, so a captured call may be replayed
- * with other offsets.  offsets must not decrease; parts of them outside 0 .. rows are cut off.  Rows of y before
+ * with other offsets.  Parts of the offsets outside 0 .. rows are cut off.  They must not decrease: rows of y that two
+ * experts then claim, or that only wrapped sums reach, are undefined, but nothing else is touched.  Rows of y before
  * offsets[0] and from offsets[experts] on are left as they were.  A row whose src (without src: r itself) is outside
  * 0 .. x_rows - 1 is taken as a row of zeros.  int8 sums are exact int32 (k <= 131071); the others are float32. */
 typedef struct {
@@ -399,7 +400,7 @@ typedef struct {
     const float *bias;        /* [experts][n] or NULL                                                     */
     const float *row_scale;   /* [rows] or NULL                                                           */
     size_t ldx, ldy, ldw, w_stride;
-    int rows, x_rows, experts, n, k;  /* experts <= 1024, k <= 2^28                                       */
+    int rows, x_rows, experts, n, k;  /* experts <= 1024, n and k <= 2^28                                 */
     int type;                 /* QCNN_F32, QCNN_F16, QCNN_BF16 or QCNN_I8                                 */
     int out_type;             /* QCNN_F32, QCNN_F16 or QCNN_BF16                                          */
     int act;                  /* QCNN_ACT_*                                                               */

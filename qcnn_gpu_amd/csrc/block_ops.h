@@ -53,7 +53,7 @@ __device__ __forceinline__ void store_typed(void *p, size_t i, int type, float v
 
 __device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + __expf(-v)); }
 
-// ReLU as the library's layers have it, with NaN kept; SiLU v * sigmoid(v), written so that -inf gives -0.
+// ReLU as the library's layers have it, with NaN kept; SiLU v * sigmoid(v), -0 where e^-v overflows.
 __device__ __forceinline__ float block_act(float v, int act)
 {
     if (act == QCNN_ACT_RELU) return v < 0.f ? 0.f : v;

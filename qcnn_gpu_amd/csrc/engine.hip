@@ -1659,7 +1659,7 @@ int qcnn_op_grouped_matmul(const qcnn_grouped_matmul_t *a, void *stream)
     if (a->rows < 0 || a->x_rows < 0 || a->n < 1 || a->k < 1)
         return fail(QCNN_E_ARG, "bad shape: rows %d, x_rows %d, n %d, k %d", a->rows, a->x_rows, a->n, a->k);
     if (a->experts < 1 || a->experts > 1024) return fail(QCNN_E_UNSUPPORTED, "%d experts (1 to 1024)", a->experts);
-    if (a->k > 1 << 28) return fail(QCNN_E_UNSUPPORTED, "k %d: at most 2^28", a->k);
+    if (a->k > 1 << 28 || a->n > 1 << 28) return fail(QCNN_E_UNSUPPORTED, "n %d, k %d: at most 2^28", a->n, a->k);
     if (a->type == QCNN_I8 && a->k > 131071) return fail(QCNN_E_UNSUPPORTED, "k %d: int8 sums leave int32 beyond 131071", a->k);
     if (a->ldx < (size_t)a->k || a->ldy < (size_t)a->n || a->ldw < (size_t)a->k)
         return fail(QCNN_E_ARG, "row strides %zu, %zu, %zu are shorter than a row", a->ldx, a->ldy, a->ldw);

@@ -94,11 +94,17 @@ struct Tiles {
             const unsigned total = __builtin_amdgcn_readlane(s, 63);
             if (at < (before + total) * nt) break;
             before += total;
-            e0 += 64;  // (at < all * nt: ends inside the experts)
+            e0 += 64;
+            if (e0 >= a.experts) return false;
             s = scan(a, e0, l0, h0, n);
         }
-        const int l = __ffsll(__ballot(at < (before + s) * nt)) - 1;
+        const unsigned long long at_or_behind = __ballot(at < (before + s) * nt);
+        if (!at_or_behind) return false;
+        const int l = __ffsll(at_or_behind) - 1;
         const unsigned m = __builtin_amdgcn_readlane(n, l), in = at - (before + __builtin_amdgcn_readlane(s, l) - m) * nt;
+        // Offsets that decrease can make more tiles than the grid was made for, and sums that wrap: what does not lie in the
+        // expert found is dropped (m * nt < 2^32, the host has seen to it).
+        if (in >= m * nt) return false;
         const unsigned band = in / (8 * nt), rows = min(8u, m - band * 8), rest = in - band * 8 * nt;
         t.e = e0 + l;
         t.first = __builtin_amdgcn_readlane(l0, l) + (int)(band * 8 + rest % rows) * TM;
@@ -109,8 +115,12 @@ struct Tiles {
 };
 
 // Row tiles a call can have: offsets are device memory, so the grid covers the most that `rows` allows (each expert
-// with rows ends in one short tile); workgroups without a tile leave.
-static unsigned most_tiles(const qcnn_grouped_matmul_t &a, int TM) { return (unsigned)(a.rows / TM + (a.experts < a.rows ? a.experts : a.rows)); }
+// with rows ends in one short tile); workgroups without a tile leave.  `tiles` stays below 2^31, n below 2^28.
+static hipError_t count_tiles(const qcnn_grouped_matmul_t &a, int TM, int TN, unsigned long long &tiles)
+{
+    tiles = ((unsigned long long)(a.rows / TM) + (a.experts < a.rows ? a.experts : a.rows)) * ((a.n + TN - 1) / TN);
+    return tiles < 1ull << 31 ? hipSuccess : hipErrorInvalidConfiguration;
+}
 
 // N neighbouring outputs of one row.  `least` is 0 for ReLU, else -inf (a NaN passes either way).  STREAM: past the caches.
 template <typename OT, int N, bool STREAM = false>
@@ -593,12 +603,14 @@ template <typename T, int MT, int RB, int KW, int NW, int KB>
 static hipError_t run_rows(const qcnn_grouped_matmul_t &a, bool al, hipStream_t s)
 {
     typedef RowsGeom<T, MT, RB, KW, NW, KB> G;
-    const unsigned long long tiles = (unsigned long long)most_tiles(a, 16 * MT) * ((a.n + 16 * NW - 1) / (16 * NW));
+    unsigned long long tiles;
+    hipError_t e = count_tiles(a, 16 * MT, 16 * NW, tiles);
+    if (e != hipSuccess) return e;
     const unsigned long long blocks = (tiles + 7) / 8 * 8;  // as many on each XCD
     if (blocks * (64 * KW * NW) > 0xffffffffull) return hipErrorInvalidConfiguration;
     static std::atomic<unsigned long long> asked[2] = {{0}, {0}};
     const auto fn = al ? k_grouped_rows<T, MT, RB, KW, NW, KB, true> : k_grouped_rows<T, MT, RB, KW, NW, KB, false>;
-    const hipError_t e = allow_lds((const void *)fn, G::LDS, asked[al]);
+    e = allow_lds((const void *)fn, G::LDS, asked[al]);
     if (e != hipSuccess) return e;
     fn<<<(unsigned)blocks, 64 * KW * NW, G::LDS, s>>>(a);
     return hipGetLastError();
@@ -619,7 +631,9 @@ template <typename T, int TM, int TN, int WM, int WN>
 static hipError_t run_tile(const qcnn_grouped_matmul_t &a, bool al, hipStream_t s)
 {
     constexpr int LDS = 4 * (TM + TN) * 64, PER_CU = 163840 / LDS < 8 / (WM * WN) ? 163840 / LDS : 8 / (WM * WN);
-    const unsigned long long tiles = (unsigned long long)most_tiles(a, TM) * ((a.n + TN - 1) / TN);
+    unsigned long long tiles;
+    hipError_t e = count_tiles(a, TM, TN, tiles);
+    if (e != hipSuccess) return e;
     const unsigned long long fit = (unsigned long long)compute_units() * PER_CU;
     const unsigned blocks = (unsigned)(((tiles < fit ? tiles : fit) + 7) / 8 * 8);  // as many on each XCD; they walk the tiles
     auto fn = k_grouped_tile<T, TM, TN, WM, WN, true>;
@@ -627,7 +641,7 @@ static hipError_t run_tile(const qcnn_grouped_matmul_t &a, bool al, hipStream_t 
         if (!al) fn = k_grouped_tile<T, TM, TN, WM, WN, false>;
     }
     static std::atomic<unsigned long long> asked[2] = {{0}, {0}};
-    const hipError_t e = allow_lds((const void *)fn, LDS, asked[al]);
+    e = allow_lds((const void *)fn, LDS, asked[al]);
     if (e != hipSuccess) return e;
     fn<<<blocks, 64 * WM * WN, LDS, s>>>(a);
     return hipGetLastError();
@@ -719,7 +733,10 @@ __global__ __launch_bounds__(256) void k_grouped_narrow(const qcnn_grouped_matmu
 template <typename T, int NT, int OPS, int TM>
 static hipError_t launch_narrow(const qcnn_grouped_matmul_t &a, hipStream_t s)
 {
-    const unsigned long long blocks = ((unsigned long long)most_tiles(a, TM) + 7) / 8 * 8;
+    unsigned long long tiles;
+    const hipError_t e = count_tiles(a, TM, 64, tiles);
+    if (e != hipSuccess) return e;
+    const unsigned long long blocks = (tiles + 7) / 8 * 8;
     if (blocks * 256 > 0xffffffffull) return hipErrorInvalidConfiguration;
     k_grouped_narrow<T, NT, OPS, TM><<<(unsigned)blocks, 256, 0, s>>>(a);
     return hipGetLastError();

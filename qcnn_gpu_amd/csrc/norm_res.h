@@ -179,7 +179,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void k_norm_res(const qcnn_n
     constexpr bool EARLY = CPT * LPR <= 2048;
     C xr[EARLY ? CPT : 1], gr[EARLY ? CPT : 1];
     const T *x = (const T *)a.x + r * a.ldx;
-    const T *g = a.gate ? (const T *)a.gate + (r / (unsigned)a.gate_rows) * a.ldg : nullptr;
+    const T *g = a.gate ? (const T *)a.gate + ((unsigned)r / (unsigned)a.gate_rows) * a.ldg : nullptr;
 #pragma unroll
     for (int c = 0; c < CPT; ++c) {
         const int at = (c * LPR + t) * VE;
@@ -269,11 +269,12 @@ static hipError_t run(const qcnn_norm_res_t &a, hipStream_t s)
     // takes as long either way (4096 x 1024 and two readers 18.8 -> 17.8, 16384 x 4096 207 -> 206), but finds smaller ones sooner in
     // the caches (256 x 4096 and two readers 11.6, 12.0 past them).
     const bool stream = (size_t)a.rows * a.d * sizeof(T) * ((a.h != nullptr) + (a.n != nullptr)) >= (size_t)8 << 20;
-    const unsigned blocks = (unsigned)((a.rows + RPB - 1) / RPB);
+    const unsigned long long blocks = ((unsigned long long)a.rows + RPB - 1) / RPB;
+    if (blocks * BLOCK > 0xffffffffull) return hipErrorInvalidConfiguration;
     if (stream)
-        k_norm_res<T, LPR, CPT, true><<<blocks, BLOCK, 0, s>>>(a);
+        k_norm_res<T, LPR, CPT, true><<<(unsigned)blocks, BLOCK, 0, s>>>(a);
     else
-        k_norm_res<T, LPR, CPT, false><<<blocks, BLOCK, 0, s>>>(a);
+        k_norm_res<T, LPR, CPT, false><<<(unsigned)blocks, BLOCK, 0, s>>>(a);
     return hipGetLastError();
 }
 

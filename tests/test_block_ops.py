@@ -36,7 +36,7 @@ REFUSED = [
     (grouped, dict(type=4), E_UNSUPPORTED), (grouped, dict(out_type=capi.I8), E_UNSUPPORTED), (grouped, dict(act=3), E_ARG), (grouped, dict(act=-1), E_ARG),
     (grouped, dict(rows=-1), E_ARG), (grouped, dict(x_rows=-1, src=A), E_ARG), (grouped, dict(n=0), E_ARG),
     (grouped, dict(k=0), E_ARG), (grouped, dict(experts=0), E_UNSUPPORTED), (grouped, dict(experts=1025), E_UNSUPPORTED),
-    (grouped, dict(k=(1 << 28) + 1, ldx=1 << 29, ldw=1 << 29), E_UNSUPPORTED), (grouped, dict(type=capi.I8, k=131072, ldx=131072, ldw=131072), E_UNSUPPORTED), (grouped, dict(ldx=63), E_ARG), (grouped, dict(ldy=7), E_ARG),
+    (grouped, dict(k=(1 << 28) + 1, ldx=1 << 29, ldw=1 << 29), E_UNSUPPORTED), (grouped, dict(n=(1 << 28) + 1, ldy=1 << 29), E_UNSUPPORTED), (grouped, dict(type=capi.I8, k=131072, ldx=131072, ldw=131072), E_UNSUPPORTED), (grouped, dict(ldx=63), E_ARG), (grouped, dict(ldy=7), E_ARG),
     (grouped, dict(ldw=63), E_ARG), (grouped, dict(w_stride=1 << 62), E_ARG), (grouped, dict(x=None), E_ARG), (grouped, dict(w=None), E_ARG),
     (grouped, dict(y=None), E_ARG), (grouped, dict(offsets=None), E_ARG), (grouped, dict(offsets=A + 2), E_ARG), (grouped, dict(src=A + 1), E_ARG),
     (grouped, dict(x=A + 1), E_ARG), (grouped, dict(bias=A + 2), E_ARG), (grouped, dict(row_scale=A + 2), E_ARG),

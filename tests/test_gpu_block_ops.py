@@ -173,7 +173,8 @@ def grouped_run(sizes, n, k, kind, okind, seed, gather=False, scales=False, bias
                                            np.full((rows, n), PAD))
     y = yv[:, :n].double().cpu().numpy()
     lo, hi = max(0, int(off[0])), min(rows, int(off[-1]))
-    assert (y[:lo] == PAD).all() and (y[max(lo, hi):] == PAD).all()  # rows of no expert stay
+    if (off[1:] >= off[:-1]).all():
+        assert (y[:lo] == PAD).all() and (y[max(lo, hi):] == PAD).all()  # rows of no expert stay
     return yv[:, :n], want, bound
 
 
@@ -237,6 +238,98 @@ def test_grouped_offsets_are_cut_to_the_rows(offsets):
     """sizes give 40 rows; offsets outside are cut off, rows of no expert stay."""
     for kind in ("bf16", "f32"):
         close(*grouped_run([13, 13, 14], 36, 64, kind, "f32", 1, offsets=offsets), "f32")
+
+
+@pytest.mark.parametrize("kind", ("bf16", "i8", "f32"))
+def test_grouped_decreasing_offsets_touch_nothing_else(kind):
+    """Offsets that break the contract: rows may hold anything, nothing outside y's rows is written (grouped_run looks)."""
+    for sizes, n, k in (([40] * 5, 70, 64), ([700] * 3, 300, 64), ([900] * 3, 30, 48)):
+        rows = sum(sizes)
+        for off in ([0, rows, 5, rows, 0, rows], [rows, 0, rows, 0, rows, 0], [7, 3, 1, 0, -5, -9]):
+            grouped_run(sizes, n, k, kind, "f32", 3, offsets=off[:len(sizes) + 1])
+
+
+@pytest.mark.parametrize("experts", (64, 65, 300, 1024))
+def test_grouped_many_experts(experts):
+    """The offsets are summed up 64 experts at a time."""
+    sizes = [(i * 7 + 3) % 4 if i % 5 else 0 for i in range(experts)]
+    close(*grouped_run(sizes, 40, 32, "bf16", "f32", experts, gather=True, bias=True), "f32")
+    sizes = [0] * experts
+    sizes[-1], sizes[experts // 2] = 300, 200
+    close(*grouped_run(sizes, 136, 64, "f16", "f32", experts, bias=True), "f32")
+
+
+def test_grouped_nan_stays_in_its_row_and_its_output():
+    """A NaN or infinity in a row of x or of w reaches that row's or that output's values alone, whatever kernel runs."""
+    for sizes, n, k in (([3, 2], 40, 96), ([70, 90], 200, 64), ([300, 900], 60, 40)):
+        g = torch.Generator().manual_seed(n)
+        rows, e = sum(sizes), len(sizes)
+        x, w = torch.randn(rows, k, generator=g).bfloat16().cuda(), torch.randn(e, n, k, generator=g).bfloat16().cuda()
+        x[1, 5], x[rows - 1, k - 1], w[1, 7, 3] = float("nan"), float("inf"), float("nan")
+        y = torch.zeros(rows, n, device="cuda")
+        off = torch.tensor([0] + sizes).cumsum(0).to(torch.int32).cuda()
+        call(capi.load().qcnn_op_grouped_matmul, capi.GroupedMatmul(x=ptr(x), y=ptr(y), w=ptr(w), offsets=ptr(off), ldx=k, ldy=n, ldw=k, w_stride=n * k, rows=rows,
+             x_rows=rows, experts=e, n=n, k=k, type=capi.BF16, out_type=capi.F32))
+        bad = ~torch.isfinite(y)
+        want = torch.zeros_like(bad)
+        want[1], want[rows - 1] = True, True
+        want[sizes[0]:, 7] = True
+        assert torch.equal(bad, want)
+
+
+def test_half_subnormals_are_multiplied():
+    """Half inputs below 2^-14 keep their value in the matrix instructions."""
+    x = torch.full((4, 64), 3e-6, dtype=torch.float64)
+    w = torch.full((33, 32), 0x99, dtype=torch.uint8)  # codes of 1
+    y, want, bound = w4_run(x, w, torch.ones(1, 33, dtype=torch.float64), None, None, 64, "f16", okind="f32")
+    close(y, want, bound, "f32")
+    assert (y > 1.8e-4).all()
+    xh, wh = x.half().cuda(), torch.ones(1, 40, 64, dtype=torch.float16, device="cuda")
+    out, off = torch.zeros(4, 40, device="cuda"), torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    call(capi.load().qcnn_op_grouped_matmul, capi.GroupedMatmul(x=ptr(xh), y=ptr(out), w=ptr(wh), offsets=ptr(off), ldx=64, ldy=40, ldw=64, w_stride=40 * 64, rows=4,
+         x_rows=4, experts=1, n=40, k=64, type=capi.F16, out_type=capi.F32))
+    assert torch.allclose(out, xh.float().sum(1, keepdim=True).expand(4, 40), rtol=1e-5, atol=0)
+
+
+# ---- addresses beyond 32 bits -----------------------------------------------------------------------------
+def test_w4_far_addresses():
+    n, k, rows = 70000, 131072, 2  # 4.6 GB of codes
+    g = torch.Generator().manual_seed(1)
+    w = torch.empty(n, k // 2, dtype=torch.uint8, device="cuda")
+    last = torch.randint(0, 256, (3, k // 2), generator=g, dtype=torch.uint8)
+    w[-3:] = last.cuda()
+    x, s = torch.randn(rows, k, generator=g).bfloat16().cuda(), (torch.rand(k // 128, n, generator=g) / 512).cuda()
+    y = torch.zeros(rows, n, device="cuda")
+    call(capi.load().qcnn_op_matvec_w4, capi.MatvecW4(x=ptr(x), y=ptr(y), w=ptr(w), scale=ptr(s), ldx=k, ldy=n, ldw=k // 2, rows=rows, n=n, k=k, group=128,
+         type=capi.BF16, scale_type=capi.F32, out_type=capi.F32))
+    want, bound = np_blocks.matvec_w4(np64(x), last.numpy(), np64(s[:, -3:]), None, None, k, 128)
+    close(y[:, -3:], want, bound, "f32")
+
+
+def test_grouped_far_addresses():
+    e, n, k = 40, 8192, 8192  # 5.4 GB of weights; and rows of x and y 2.2 GB apart
+    g = torch.Generator().manual_seed(2)
+    w = torch.empty(e, n, k, dtype=torch.bfloat16, device="cuda")
+    w[-1, -2:] = (torch.randn(2, k, generator=g) / 64).bfloat16().cuda()
+    x = torch.empty(3, 1 << 30, dtype=torch.bfloat16, device="cuda")
+    x[:, :k] = torch.randn(3, k, generator=g).bfloat16().cuda()
+    y = torch.empty(3, 1 << 30, dtype=torch.bfloat16, device="cuda")
+    off = torch.zeros(e + 1, dtype=torch.int32, device="cuda")
+    off[-1] = 3
+    call(capi.load().qcnn_op_grouped_matmul, capi.GroupedMatmul(x=ptr(x), y=ptr(y), w=ptr(w), offsets=ptr(off), ldx=1 << 30, ldy=1 << 30, ldw=k, w_stride=n * k, rows=3,
+         x_rows=3, experts=e, n=n, k=k, type=capi.BF16, out_type=capi.BF16))
+    want, bound = np_blocks.grouped_matmul(np64(x[:, :k]), np64(w[-1:, -2:]), [0, 3], None, None, None, None, None, 0, np.zeros((3, 2)))
+    close(y[:, n - 2:n], want, bound, "bf16")
+
+
+def test_norm_far_addresses():
+    rows, d = 40000, 65536  # 5.2 GB a buffer
+    x, n = (torch.empty(rows, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    x[-1] = torch.randn(d, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    call(capi.load().qcnn_op_norm_res, capi.NormRes(x=ptr(x), n=ptr(n), ldx=d, ldn=d, rows=rows, d=d, parts=1, type=capi.BF16, w_type=capi.F32, pre=1, beta=1.0,
+         pre_eps=1e-6))
+    _, _, want, bound = np_blocks.norm_res(np64(x[-1:]), None, None, None, 1, 0, None, None, 1, None, None, 0, 0, 1, 0, 1e-6, 0)
+    close(n[-1:], want, bound, "bf16")
 
 
 # ---- the two ends of a residual block ---------------------------------------------------------------------
