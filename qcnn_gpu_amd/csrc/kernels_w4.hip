@@ -9,8 +9,9 @@
 // The waves of a workgroup are KW x NW: NW share out the outputs, 16 NT each, KW the k, in runs of 128, and the KW sums
 // meet in LDS at the end.  Everything goes through LDS, brought there by direct loads R - 1 runs ahead of its use, so that
 // a wave has kilobytes on their way without registers for them.  A wave issues an instruction every seven cycles or so, so
-// instructions a run and waves on a CU set the pace where the memory does not.  A wave brings its own codes and scales; x is shared by the NW waves of a k group, one
-// barrier a run, none for NW = 1.
+// instructions a run and waves on a CU set the pace where the memory does not.  A wave brings its own codes and scales; x is
+// shared by the NW waves of a k group, one barrier a run, none for NW = 1.
+// Measured: 16 half rows, 16384 x 8192, groups of 64 with zeros: 21 us, 3.5 TB/s; one bfloat16 row, 4096 x 4096: 4.6 us.
 // Of 128 k a lane holds 16 bytes of each of its weight rows: lane l, row l & 15, k from (l >> 4) * 32 on.  Instruction j
 // of four wants k = 32 j + (l >> 4) * 8 there, so that its 32 k lie in one group: a 4 x 4 transposition of dwords among
 // the lanes l, l + 16, l + 32, l + 48, four swaps of rows of lanes.

