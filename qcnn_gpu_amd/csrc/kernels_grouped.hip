@@ -2,6 +2,8 @@
 //   y[r][j] = row_scale[r] * act(w_scale[e][j] * x_scale[s] * sum_k w[e][j][k] * x[s][k] + bias[e][j]),  s = src[r].
 #include "block_ops.h"
 
+#include <type_traits>
+
 namespace qcnn {
 
 typedef u32x4 u32x4_any __attribute__((aligned(1)));  // global loads and stores take any address
@@ -42,9 +44,9 @@ __device__ __forceinline__ f32x4 mma(float, u32x4 a, u32x4 b, f32x4 c)
     return c;
 }
 
-// A tile of TM rows of one expert and TN outputs.
+// A tile of TM rows of one expert and TN outputs, or (parts = 2) half of its rows.
 struct Tile {
-    int e, first, count, n0;
+    int e, first, count, n0, parts;
 };
 
 // The tiles of a call.  They are counted through the experts in turn; workgroups are dealt to the 8 XCDs round robin
@@ -52,7 +54,11 @@ struct Tile {
 // after the other, and inside an expert the order walks bands of 8 row tiles column by column: the 32 workgroups that
 // run on an XCD at a time then share 8 row tiles of x and 4 column tiles of w.
 // The offsets are device memory, so each wave adds up the tiles itself, 64 experts at a time over its lanes.
-template <int TM, int TN>
+// PARTS = 2: a tile of at most half of its rows is made as a half, and where the last round of an XCD's workgroups, PER_CU
+// on a CU, would leave half of its CUs idle, its tiles are cut in halves (4096 rows over 8, 2048 x 4096 bfloat16 129 -> 123 us,
+// 16384 over 16, 4096 x 2048 336 -> 327, int8 8192 over 8, 4096 x 4096 198 -> 192; quarters, and halves of 64 x 64 tiles,
+// were no faster).
+template <int TM, int TN, int PARTS = 1, int PER_CU = 1>
 struct Tiles {
     unsigned all, nt;  // row tiles of all experts, column tiles
 
@@ -86,7 +92,17 @@ struct Tiles {
     // the i-th tile of this workgroup's XCD, false beyond the last
     __device__ __forceinline__ bool get(const qcnn_grouped_matmul_t &a, unsigned i, Tile &t) const
     {
-        const unsigned per = (all * nt + 7) / 8, at = (blockIdx.x & 7) * per + i;
+        const unsigned per = (all * nt + 7) / 8;
+        unsigned piece = 0, pieces = 1;
+        if constexpr (PARTS > 1) {
+            const unsigned walkers = gridDim.x >> 3, whole = per / walkers * walkers, left = per - whole;
+            if (i >= whole) {
+                pieces = left * PARTS * PER_CU > walkers ? 1 : PARTS;
+                piece = (i - whole) % pieces;
+                i = whole + (i - whole) / pieces;
+            }
+        }
+        const unsigned at = (blockIdx.x & 7) * per + i;
         if (i >= per || at >= all * nt) return false;
         int l0, h0, e0 = 0;
         unsigned n, s = scan(a, 0, l0, h0, n), before = 0;
@@ -107,10 +123,11 @@ struct Tiles {
         if (in >= m * nt) return false;
         const unsigned band = in / (8 * nt), rows = min(8u, m - band * 8), rest = in - band * 8 * nt;
         t.e = e0 + l;
-        t.first = __builtin_amdgcn_readlane(l0, l) + (int)(band * 8 + rest % rows) * TM;
-        t.count = min(TM, (int)__builtin_amdgcn_readlane(h0, l) - t.first);
+        t.first = __builtin_amdgcn_readlane(l0, l) + (int)(band * 8 + rest % rows) * TM + (int)(piece * (TM / pieces));
+        t.count = min((int)(TM / pieces), (int)__builtin_amdgcn_readlane(h0, l) - t.first);
         t.n0 = (int)(rest / rows) * TN;
-        return true;
+        t.parts = t.count <= TM / PARTS ? PARTS : 1;
+        return t.count > 0;  // (a part without rows: of the last round)
     }
 };
 
@@ -248,10 +265,16 @@ __device__ __forceinline__ void load_to_lds(const char *from, unsigned lds)
 // Measured with tiles of 256 x 256, one expert: 8192 x 8192 x 8192 1214 TFLOP/s in bfloat16 and 2270 TOP/s in int8, where
 // the power limit holds the clock; 16 experts of 1024 rows, 4096 x 2048: 1040, the epilogues and the ragged last round take
 // the rest.
+template <int TM, int TN, int WM, int WN>
+struct TileGeom {
+    static constexpr int LDS = 4 * (TM + TN) * 64, PER_CU = 163840 / LDS < 8 / (WM * WN) ? 163840 / LDS : 8 / (WM * WN);
+    static constexpr int PARTS = TM >= 128 ? 2 : 1;
+};
+
 template <typename T, int TM, int TN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grouped_matmul_t a)
 {
-    constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+    constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, PARTS = TileGeom<TM, TN, WM, WN>::PARTS;
     constexpr int FM = TM / WM / 16, FN = TN / WN / 16;             // 16 x 16 tiles of a wave
     constexpr int LX = TM * 4 / THREADS, LW = TN * 4 / THREADS;     // chunks a thread loads in one step
     constexpr int BUF = (TM + TN) * 64;
@@ -260,9 +283,9 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grou
     typedef typename Mma<T>::acc_t acc_t;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    Tiles<TM, TN> tiles;
+    Tiles<TM, TN, PARTS, TileGeom<TM, TN, WM, WN>::PER_CU> tiles;
     tiles.count(a);
-    Tile t{0, 0, 0, 0}, next_t;
+    Tile t{0, 0, 0, 0, 1}, next_t;
     unsigned index = blockIdx.x >> 3;
     if (!tiles.get(a, index, t)) return;
 
@@ -286,30 +309,30 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grou
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char *)lds;
     const int steps = (bytes + 63) / 64;
     u32x4 held[ALIGNED ? 1 : LX + LW];
-    // asks for chunk i of the thread's LX + LW of a step; called step after step, the pointers walk
-    const auto request_one = [&](int step, int i, bool ended) {
-        const char *&p = i < LX ? xp[i < LX ? i : 0] : wp[i < LX ? 0 : i - LX];
-        const unsigned at = lds0 + (step & 3) * BUF + wave * 1024 + (i < LX ? i * (THREADS * 16) : TM * 64 + (i - LX) * (THREADS * 16));
+    // asks for chunk i of the thread's lx + LW of a step; called step after step, the pointers walk
+    const auto request_one = [&](int lx, int step, int i, bool ended) {
+        const char *&p = i < lx ? xp[i < lx ? i : 0] : wp[i < lx ? 0 : i - lx];
+        const unsigned at = lds0 + (step & 3) * BUF + wave * 1024 + (i < lx ? i * (THREADS * 16) : TM * 64 + (i - lx) * (THREADS * 16));
         load_to_lds(ended ? (const char *)&k_zero_chunk : p, at);
         p += 64;
     };
-    const auto request = [&](int step) {
+    const auto request = [&](auto lx, int step) {
         if constexpr (ALIGNED) {
             const bool ended = step * 64 + chunk >= bytes;
 #pragma unroll
-            for (int i = 0; i < LX + LW; ++i) request_one(step, i, ended);
+            for (int i = 0; i < lx() + LW; ++i) request_one(lx(), step, i, ended);
         } else {
 #pragma unroll
-            for (int i = 0; i < LX; ++i) held[i] = load_chunk(xp[i], step * 4 + chunk / 16, bytes);
+            for (int i = 0; i < lx(); ++i) held[i] = load_chunk(xp[i], step * 4 + chunk / 16, bytes);
 #pragma unroll
             for (int i = 0; i < LW; ++i) held[LX + i] = load_chunk(wp[i], step * 4 + chunk / 16, bytes);
         }
     };
-    const auto deposit = [&](int step) {
+    const auto deposit = [&](auto lx, int step) {
         if constexpr (!ALIGNED) {
             char *at = lds + (step & 3) * BUF + tid * 16;
 #pragma unroll
-            for (int i = 0; i < LX; ++i) *(u32x4 *)(at + i * (THREADS * 16)) = held[i];
+            for (int i = 0; i < lx(); ++i) *(u32x4 *)(at + i * (THREADS * 16)) = held[i];
 #pragma unroll
             for (int i = 0; i < LW; ++i) *(u32x4 *)(at + TM * 64 + i * (THREADS * 16)) = held[LX + i];
         }
@@ -317,67 +340,80 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grou
 
     const int wm = wave % WM, wn = wave / WM, c16 = lane & 15, g = lane >> 4;
     const int from = c16 * 64 + (g ^ swizzle(c16)) * 16;  // rows of a wave's tiles begin at multiples of 16
-    u32x4 fw[FN], fx[2][FM];  // a step's operands; w of the next step takes the place of what has been used
-    const auto read_w = [&](int step, int j) { fw[j] = *(const u32x4 *)(lds + (step & 3) * BUF + from + TM * 64 + wn * (TN / WN) * 64 + j * 1024); };
-    const auto read_x = [&](int step, u32x4(&x)[FM], int i) { x[i] = *(const u32x4 *)(lds + (step & 3) * BUF + from + wm * (TM / WM) * 64 + i * 1024); };
-    const auto read = [&](int step) {
-#pragma unroll
-        for (int j = 0; j < FN; ++j) read_w(step, j);
-#pragma unroll
-        for (int i = 0; i < FM; ++i) read_x(step, fx[0], i);
+    const auto with_parts = [&](int parts, auto f) {
+        parts = __builtin_amdgcn_readfirstlane(parts);
+        if constexpr (PARTS > 1) {
+            if (parts == PARTS) return f(std::integral_constant<int, PARTS>());
+        }
+        f(std::integral_constant<int, 1>());
     };
-    acc_t acc[FN][FM];
-    const auto multiply_part = [&](const u32x4(&x)[FM], int j) {
-#pragma unroll
-        for (int i = 0; i < FM; ++i) acc[j][i] = mma(T(), fw[j], x[i], acc[j][i]);
-    };
-    const auto multiply = [&](const u32x4(&x)[FM]) {
-#pragma unroll
-        for (int j = 0; j < FN; ++j) multiply_part(x, j);
-    };
-    // (ALIGNED) The chunks of step s have landed, here and (after the barrier) everywhere, and everyone has read step s - 1
-    // into registers.  Loads land in order, so all but those of the two steps behind s are waited for.
-    const auto arrive = [&](int s) {
-        if (s + 2 < steps)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * (LX + LW)) : "memory");
-        else if (s + 1 < steps)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LX + LW) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    };
+    // chunks of x that a thread asks for in one step, at least one: those of rows that do not count are the last row's
+    const auto chunks_of = [](auto parts) { return std::integral_constant<int, (LX / parts() > 0 ? LX / parts() : 1)>(); };
 
-    const auto begin = [&] {
-        request(0);
+    const auto begin = [&](auto lx) {
+        request(lx, 0);
         if constexpr (ALIGNED) {
-            if (1 < steps) request(1);
-            if (2 < steps) request(2);
+            if (1 < steps) request(lx, 1);
+            if (2 < steps) request(lx, 2);
         }
     };
     rows_of(t);
-    begin();
-    for (;;) {
+    with_parts(t.parts, [&](auto p) { begin(chunks_of(p)); });
+    bool more = false;
+    const auto product = [&](auto parts) {
+        constexpr int M = FM / parts(), L = decltype(chunks_of(parts))::value;
+        constexpr std::integral_constant<int, L> lx;
+        u32x4 fw[FN], fx[2][M];  // a step's operands; w of the next step takes the place of what has been used
+        const auto read_w = [&](int step, int j) { fw[j] = *(const u32x4 *)(lds + (step & 3) * BUF + from + TM * 64 + wn * (TN / WN) * 64 + j * 1024); };
+        const auto read_x = [&](int step, u32x4(&x)[M], int i) { x[i] = *(const u32x4 *)(lds + (step & 3) * BUF + from + wm * (M * 16) * 64 + i * 1024); };
+        const auto read = [&](int step) {
+#pragma unroll
+            for (int j = 0; j < FN; ++j) read_w(step, j);
+#pragma unroll
+            for (int i = 0; i < M; ++i) read_x(step, fx[0], i);
+        };
+        acc_t acc[FN][M];
+        const auto multiply_part = [&](const u32x4(&x)[M], int j) {
+#pragma unroll
+            for (int i = 0; i < M; ++i) acc[j][i] = mma(T(), fw[j], x[i], acc[j][i]);
+        };
+        const auto multiply = [&](const u32x4(&x)[M]) {
+#pragma unroll
+            for (int j = 0; j < FN; ++j) multiply_part(x, j);
+        };
+        // (ALIGNED) The chunks of step s have landed, here and (after the barrier) everywhere, and everyone has read step s - 1
+        // into registers.  Loads land in order, so all but those of the two steps behind s are waited for.
+        const auto arrive = [&](int s) {
+            if (s + 2 < steps)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * (L + LW)) : "memory");
+            else if (s + 1 < steps)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(L + LW) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        };
+
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
-            for (int i = 0; i < FM; ++i) acc[j][i] = acc_t{0, 0, 0, 0};
+            for (int i = 0; i < M; ++i) acc[j][i] = acc_t{0, 0, 0, 0};
         if constexpr (ALIGNED) {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (3 < steps) request(3);
+            if (3 < steps) request(lx, 3);
             read(0);
             // Matrix instructions first: their operands are there.  The reads of the next step and the requests stand between
             // groups of them, as a wave issues in order and would hold its matrix instructions up behind them: all of them in
             // front left the matrix cores idle half of the time.  No branch in here; the last steps are made below.
-            const auto step = [&](int s, u32x4(&now)[FM], u32x4(&next)[FM]) {
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * (LX + LW)) : "memory");
+            const auto step = [&](int s, u32x4(&now)[M], u32x4(&next)[M]) {
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * (L + LW)) : "memory");
 #pragma unroll
                 for (int j = 0; j < FN; ++j) {
                     multiply_part(now, j);
                     __builtin_amdgcn_sched_barrier(0);
                     read_w(s + 1, j);
 #pragma unroll
-                    for (int i = FM * j / FN; i < FM * (j + 1) / FN; ++i) read_x(s + 1, next, i);
+                    for (int i = M * j / FN; i < M * (j + 1) / FN; ++i) read_x(s + 1, next, i);
 #pragma unroll
-                    for (int i = (LX + LW) * j / FN; i < (LX + LW) * (j + 1) / FN; ++i) request_one(s + 4, i, false);
+                    for (int i = (L + LW) * j / FN; i < (L + LW) * (j + 1) / FN; ++i) request_one(L, s + 4, i, false);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
@@ -391,38 +427,41 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grou
                 multiply(fx[0]);
                 if (s + 1 < steps) {
                     arrive(s + 1);
-                    if (s + 4 < steps) request(s + 4);
+                    if (s + 4 < steps) request(lx, s + 4);
                     read(s + 1);
                 }
             }
         } else {
             // Step s: s + 1 is in LDS, s + 2 is put there and s + 3 asked for, behind the matrix instructions of s.
-            deposit(0);
-            if (1 < steps) request(1);
+            deposit(lx, 0);
+            if (1 < steps) request(lx, 1);
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             read(0);
-            if (1 < steps) deposit(1);
-            if (2 < steps) request(2);
+            if (1 < steps) deposit(lx, 1);
+            if (2 < steps) request(lx, 2);
 #pragma unroll 1
             for (int s = 0; s < steps; ++s) {
                 if (s + 1 < steps) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 multiply(fx[0]);
                 __builtin_amdgcn_sched_barrier(0);
                 if (s + 1 < steps) read(s + 1);
-                if (s + 2 < steps) deposit(s + 2);
-                if (s + 3 < steps) request(s + 3);
+                if (s + 2 < steps) deposit(lx, s + 2);
+                if (s + 3 < steps) request(lx, s + 3);
             }
         }
         // the next tile's first chunks are on their way while this one's outputs are written
         index += gridDim.x >> 3;
-        const bool more = tiles.get(a, index, next_t);
+        more = tiles.get(a, index, next_t);
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // everyone has read this tile's last chunks
             rows_of(next_t);
-            begin();
+            with_parts(next_t.parts, [&](auto p) { begin(chunks_of(p)); });
         }
         // lane: row c16 of each row tile, outputs 8 g .. 8 g + 7 of each pair of output tiles
-        epilogue(a, acc, t.e, t.first, wm * (TM / WM) + c16, t.count, t.n0 + wn * (TN / WN) + 8 * g);
+        epilogue(a, acc, t.e, t.first, wm * (M * 16) + c16, t.count, t.n0 + wn * (TN / WN) + 8 * g);
+    };
+    for (;;) {
+        with_parts(t.parts, product);
         if (!more) break;
         t = next_t;
     }
@@ -472,7 +511,7 @@ __global__ __launch_bounds__(64 * KW *NW) void k_grouped_rows(const qcnn_grouped
     const int kq = wave / NW, nq = wave % NW;
     Tiles<16 * MT, 16 * NW> tiles;
     tiles.count(a);
-    Tile t{0, 0, 0, 0};
+    Tile t{0, 0, 0, 0, 1};
     if (!tiles.get(a, blockIdx.x >> 3, t)) return;
 
     // this lane's rows: one of w and, for each operand of x that this wave brings, one of x
@@ -633,20 +672,20 @@ static int compute_units()
 template <typename T, int TM, int TN, int WM, int WN>
 static hipError_t run_tile(const qcnn_grouped_matmul_t &a, bool al, hipStream_t s)
 {
-    constexpr int LDS = 4 * (TM + TN) * 64, PER_CU = 163840 / LDS < 8 / (WM * WN) ? 163840 / LDS : 8 / (WM * WN);
+    typedef TileGeom<TM, TN, WM, WN> G;
     unsigned long long tiles;
     hipError_t e = count_tiles(a, TM, TN, tiles);
     if (e != hipSuccess) return e;
-    const unsigned long long fit = (unsigned long long)compute_units() * PER_CU;
-    const unsigned blocks = (unsigned)(((tiles < fit ? tiles : fit) + 7) / 8 * 8);  // as many on each XCD; they walk the tiles
+    const unsigned long long fit = (unsigned long long)compute_units() * G::PER_CU;
+    const unsigned blocks = (unsigned)(((tiles * G::PARTS < fit ? tiles * G::PARTS : fit) + 7) / 8 * 8);  // as many on each XCD; they walk the tiles
     auto fn = k_grouped_tile<T, TM, TN, WM, WN, true>;
     if constexpr (TM < 256) {  // (the largest tiles have no registers for loads of any address)
         if (!al) fn = k_grouped_tile<T, TM, TN, WM, WN, false>;
     }
     static std::atomic<unsigned long long> asked[2] = {{0}, {0}};
-    e = allow_lds((const void *)fn, LDS, asked[al]);
+    e = allow_lds((const void *)fn, G::LDS, asked[al]);
     if (e != hipSuccess) return e;
-    fn<<<blocks, 64 * WM * WN, LDS, s>>>(a);
+    fn<<<blocks, 64 * WM * WN, G::LDS, s>>>(a);
     return hipGetLastError();
 }
 
@@ -664,7 +703,7 @@ __global__ __launch_bounds__(256) void k_grouped_narrow(const qcnn_grouped_matmu
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
     Tiles<TM, 64> tiles;
     tiles.count(a);
-    Tile t{0, 0, 0, 0};
+    Tile t{0, 0, 0, 0, 1};
     if (!tiles.get(a, blockIdx.x >> 3, t)) return;
 
     const int bytes = a.k * (int)sizeof(T);

@@ -240,6 +240,13 @@ def test_grouped_offsets_are_cut_to_the_rows(offsets):
         close(*grouped_run([13, 13, 14], 36, 64, kind, "f32", 1, offsets=offsets), "f32")
 
 
+@pytest.mark.parametrize("kind,n,k", (("i8", 4300, 96), ("f16", 8300, 64), ("bf16", 2304, 96), ("bf16", 2300, 50), ("f32", 6300, 40)))
+@pytest.mark.parametrize("sizes", ([1500, 129, 128, 1, 900, 300, 256], [64, 2000, 65, 0, 127, 640, 128]))
+def test_grouped_halves_of_tiles(sizes, kind, n, k):
+    """Tiles of at most half of their rows, and a last round of few tiles, are made in halves."""
+    close(*grouped_run(sizes, n, k, kind, "f32", n + k, gather=True, bias=True, scales=True), "f32")
+
+
 @pytest.mark.parametrize("kind", ("bf16", "i8", "f32"))
 def test_grouped_decreasing_offsets_touch_nothing_else(kind):
     """Offsets that break the contract: rows may hold anything, nothing outside y's rows is written (grouped_run looks)."""
