@@ -460,7 +460,7 @@ static hipError_t launch(const qcnn_matvec_w4_t &a, hipStream_t s)
 {
     typedef W4<T, NT, XROWS, FL, S16, ZERO, KW, NW, KB> G;
     const unsigned nblocks = (unsigned)((a.n + 16 * NT * NW - 1) / (16 * NT * NW));
-    const unsigned long long blocks = (unsigned long long)nblocks * ((a.rows + XROWS - 1) / XROWS);
+    const unsigned long long blocks = (unsigned long long)nblocks * (((unsigned)a.rows + XROWS - 1) / XROWS);
     if (blocks * (64 * G::WAVES) > 0xffffffffull) return hipErrorInvalidConfiguration;
     const auto fn = k_w4<T, NT, XROWS, FL, S16, ZERO, KW, NW, KB>;
     static std::atomic<unsigned long long> asked{0};
