@@ -3,6 +3,10 @@
 Tolerance: the oracle's first-order bound of a float32 evaluation plus half a step of the output type; integer data pins
 the element order exactly."""
 import ctypes as C
+import pathlib
+import subprocess
+import sys
+import threading
 
 import numpy as np
 import pytest
@@ -530,6 +534,56 @@ def test_a_block_captured_and_replayed():
         torch.cuda.synchronize()
         for k in ("h0", "n0", "u", "o", "h", "n", "y"):
             assert torch.equal(other[k], s[k]), k
+
+
+def test_a_block_from_threads_at_once():
+    """Four host threads, each with a stream and buffers of its own, also through the kernels that ask for more LDS."""
+    states = [block_state(50 + i, 400 if i % 2 else 9) for i in range(4)]
+    streams, errors = [torch.cuda.Stream() for _ in states], []
+    torch.cuda.synchronize()
+
+    def work(s, st):
+        try:
+            for _ in range(10):
+                block_calls(s, st.cuda_stream)
+            st.synchronize()
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(states, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for s in states:
+        block_check(s)
+
+
+def test_two_graphs_replayed_at_once():
+    states, graphs, streams = [block_state(60 + i, 60) for i in range(2)], [], [torch.cuda.Stream() for _ in range(2)]
+    for s in states:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            block_calls(s, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        block_calls(block_state(70, 5), None)  # eager work between the replays
+    torch.cuda.synchronize()
+    for s in states:
+        block_check(s)
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    code = ("import sys, torch; sys.path[:0] = ['tests', '.']; import test_gpu_block_ops as t; s = t.block_state(80, 7); g = torch.cuda.CUDAGraph()\n"
+            "with torch.cuda.graph(g): t.block_calls(s, torch.cuda.current_stream().cuda_stream)\n"
+            "for _ in range(3): g.replay(); torch.cuda.synchronize(); t.block_check(s); t.block_calls(s, None); torch.cuda.synchronize(); t.block_check(s)\n"
+            "print('checked')")
+    done = subprocess.run([sys.executable, "-c", code], cwd=pathlib.Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and done.stdout.strip().endswith("checked"), done.stderr[-2000:]
 
 
 def test_the_same_call_gives_the_same_bits():
