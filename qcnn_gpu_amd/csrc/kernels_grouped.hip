@@ -803,10 +803,14 @@ static hipError_t pick(qcnn_grouped_matmul_t a, hipStream_t s)
     //   narrow    798720 rows 48 -> 32 int8            33, tiles 136
     //   rows      64 over 64 experts, 1024 x 2048      34, 128 x 128 tiles 53;  7 rows 157 x 3840: 8 k groups 8.5, 4 26
     //             128 over 16, 2048 x 2048             30, 16 rows a workgroup 36;  200 over 8, 300 x 1000: 7.5, 64 x 64 tiles 8.8
+    //             float32 400 over 8, 300 x 2001        23, 64 x 64 tiles 93;  500 of one, 900 x 1024: 22, 64 x 64 24
     //   64 x 64   1024 over 16, 1024 x 1024            13, 128 x 128 20;  512 over 4, 1024 x 1024: 9.5, rows 20;
     //             float32 5000 over 5, 1000 x 2000    201, 128 x 128 254
+    //             float32 1000 of one, 800 x 1000      26, rows 37
     //   128 x 128 8900 over 22, 1424 x 1944           134, 256 x 256 167;  8192 over 64, 2048 x 2048: 176, 256 x 256 216
-    //   256 x 256 16384 over 16, 4096 x 2048          337, 128 x 128 403;  int8 6000 over 8, 2048 x 2048: 39, 128 x 128 47
+    //             short k: 16384 over 8, 1024 x 512     37, 256 x 256 41;  int8 8192 over 16, 2048 x 1024: 37, 256 x 256 42
+    //   256 x 256 16384 over 16, 4096 x 2048          327, 128 x 128 403;  int8 6000 over 8, 2048 x 2048: 40, 128 x 128 49
+    //             4096 of one, 4096 x 4096            119, 128 x 128 165;  16384 over 16, 1024 x 2048: 93, 128 x 128 98
     const long long groups = a.rows < a.experts ? a.rows : a.experts, avg = a.rows / a.experts;
     const auto tiles = [&](long long tm, long long tn) { return (a.rows / tm + groups) * ((a.n + tn - 1) / tn); };
     if (a.n <= 64 && a.k * z <= 256 && avg >= 512) {
@@ -817,11 +821,11 @@ static hipError_t pick(qcnn_grouped_matmul_t a, hipStream_t s)
     if (tiles(32, 32) < 128) return run_rows<T, 1, 256, 8, 1, 160>(a, al, s);
     if (avg <= 24 && a.k * z <= 512) return run_rows<T, 1, 256, 1, 4, 40>(a, al, s);  // nothing to split k for: 61 rows over 82, 2334 x 71 int8: 11 us, split 31
     if (avg <= 4) return run_rows<T, 1, 128, 4, 2, 80>(a, al, s);
-    if (tiles(64, 64) < 64) return run_rows<T, 2, 128, 4, 2, 80>(a, al, s);
+    if (tiles(64, 64) < (sizeof(T) == 4 ? 160 : 64)) return run_rows<T, 2, 128, 4, 2, 80>(a, al, s);
     if (avg <= 24) return run_rows<T, 4, 128, 2, 4, 80>(a, al, s);
     if (tiles(128, 128) < (sizeof(T) == 4 ? 1024 : 256)) return run_tile<T, 64, 64, 2, 2>(a, al, s);
     if constexpr (sizeof(T) < 4) {
-        if (al && avg >= 256 && tiles(256, 256) >= (sizeof(T) == 1 ? 240 : 512)) return run_tile<T, 256, 256, 2, 4>(a, al, s);
+        if (al && avg >= 256 && tiles(256, 256) >= (a.k >= 2048 ? 240 : 512)) return run_tile<T, 256, 256, 2, 4>(a, al, s);
     }
     return run_tile<T, 128, 128, 2, 2>(a, al, s);
 }
