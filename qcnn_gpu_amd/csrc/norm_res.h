@@ -143,15 +143,18 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void k_norm_res(const qcnn_n
     const float inv_d = 1.f / (float)d;
     float v[CPT][VE];
 
+    // (What v holds behind the row's end is not zero once a norm has subtracted a mean there: the sums leave it out.)
     const auto norm = [&](int kind, const void *w, const void *b, float eps) {
         if (kind == QCNN_NORM_NONE) return;
         float mean = 0.f;
         if (kind == QCNN_NORM_LAYER) {
             float s = 0.f;
 #pragma unroll
-            for (int c = 0; c < CPT; ++c)
+            for (int c = 0; c < CPT; ++c) {
+                const int left = d - (c * LPR + t) * VE;
 #pragma unroll
-                for (int i = 0; i < VE; ++i) s += v[c][i];
+                for (int i = 0; i < VE; ++i) s += i < left ? v[c][i] : 0.f;
+            }
             mean = row_sum<LPR>(s, red, turn) * inv_d;
         }
         float q = 0.f;
