@@ -389,7 +389,8 @@ enum { QCNN_ACT_NONE = 0, QCNN_ACT_RELU = 1, QCNN_ACT_SILU = 2 };
  * with other offsets.  Parts of the offsets outside 0 .. rows are cut off.  They must not decrease: rows of y that two
  * experts then claim, or that only wrapped sums reach, are undefined, but nothing else is touched.  Rows of y before
  * offsets[0] and from offsets[experts] on are left as they were.  A row whose src (without src: r itself) is outside
- * 0 .. x_rows - 1 is taken as a row of zeros.  int8 sums are exact int32 (k <= 131071); the others are float32. */
+ * 0 .. x_rows - 1 is taken as a row of zeros: row_scale[r] * act(bias[e][j]) is left of it, whatever w and the scales hold.
+ * int8 sums are exact int32 (k <= 131071); the others are float32. */
 typedef struct {
     const void *x;            /* [x_rows][ldx] of `type`                                                  */
     void *y;                  /* [rows][ldy] of `out_type`                                                */

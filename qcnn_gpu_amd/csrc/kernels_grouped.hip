@@ -631,9 +631,12 @@ __global__ __launch_bounds__(64 * KW *NW) void k_grouped_rows(const qcnn_grouped
         for (int k = 0; k < KW; ++k) v += sums[k * (OUT * 16 * MT) + o];
         const int r = t.first + row, s = a.src ? a.src[r] : r;
         const size_t e = (size_t)t.e * a.n + n;
-        float f = s >= 0 && s < a.x_rows ? (float)v : 0.f;
-        if (a.w_scale) f *= a.w_scale[e];
-        if (a.x_scale && s >= 0 && s < a.x_rows) f *= a.x_scale[s];
+        float f = 0.f;
+        if (s >= 0 && s < a.x_rows) {  // of another row what was summed up is dropped
+            f = (float)v;
+            if (a.w_scale) f *= a.w_scale[e];
+            if (a.x_scale) f *= a.x_scale[s];
+        }
         if (a.bias) f += a.bias[e];
         f = block_act(f, a.act);
         if (a.row_scale) f *= a.row_scale[r];

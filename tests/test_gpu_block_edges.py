@@ -8,6 +8,7 @@ from qcnn_gpu_amd import capi
 from test_gpu_block_ops import KIND, T, call, close, np64, ptr
 
 pytestmark = pytest.mark.gpu
+NAN, INF = float("nan"), float("inf")
 
 
 # ---- the end of a row between two norms ------------------------------------------------------------------
@@ -31,3 +32,42 @@ def test_layer_norm_behind_layer_norm(d, kind):
         want = np_blocks.norm_res(np64(x), np64(y), None, np64(gv), max(1, gate), 2, *map(np64, v[:2]), 2, *map(np64, v[2:]), act, 0.8, 1.0, 1e-5, 1e-5, offset)
         close(h, want[0], want[1], kind, ("h", seed))
         close(n, want[2], want[3], kind, ("n", seed))
+
+
+# ---- rows that are not there, scales that are not finite -------------------------------------------------
+@pytest.mark.parametrize("kind", ("bf16", "i8"))
+@pytest.mark.parametrize("sizes,n,k", (([3, 5], 40, 96), ([4] * 40, 300, 700), ([20] * 30, 600, 256), ([20] * 30, 600, 600), ([300, 200], 200, 130), ([300, 200, 400], 900, 130), ([600], 32, 48)), ids=str)
+def test_grouped_rows_outside_x_whatever_the_scales_hold(sizes, n, k, kind):
+    """Of a row whose src is outside x, activation and row scale of the bias are left, in every kernel: infinite or NaN weights and
+    scales are not multiplied with its zeros."""
+    g = torch.Generator().manual_seed(n)
+    e, rows = len(sizes), sum(sizes)
+    draw = (lambda *s: torch.randint(-9, 10, s, generator=g).to(torch.int8)) if kind == "i8" else (lambda *s: torch.randn(*s, generator=g).bfloat16())
+    x, w, bias = draw(rows, k).cuda(), draw(e, n, k), torch.randn(e, n, generator=g)
+    ws, rs = torch.rand(e, n, generator=g), torch.rand(rows, generator=g)
+    ws[:, 2], ws[:, 7] = INF, NAN
+    if kind == "bf16":
+        w[:, 4] = NAN
+    src = torch.arange(rows, dtype=torch.int32)
+    src[::3] = torch.tensor([-1, rows, 2 ** 31 - 1], dtype=torch.int32)[torch.arange(len(src[::3])) % 3]
+    of = torch.repeat_interleave(torch.arange(e), torch.tensor(sizes))
+    w, src, ws, bias_d, rs_d = (t.cuda() for t in (w, src, ws, bias, rs))
+    xs, off = torch.rand(rows, generator=g).cuda(), torch.tensor([0] + sizes).cumsum(0).to(torch.int32).cuda()
+    y = torch.zeros(rows, n, device="cuda")
+    call(capi.load().qcnn_op_grouped_matmul, capi.GroupedMatmul(x=ptr(x), y=ptr(y), w=ptr(w), offsets=ptr(off), src=ptr(src), x_scale=ptr(xs), w_scale=ptr(ws),
+         bias=ptr(bias_d), row_scale=ptr(rs_d), ldx=k, ldy=n, ldw=k, w_stride=n * k, rows=rows, x_rows=rows, experts=e, n=n, k=k, type=KIND[kind],
+         out_type=capi.F32, act=capi.ACT_RELU))
+    assert torch.equal(y[::3].cpu(), (bias[of].clamp_min(0) * rs[:, None])[::3])
+    assert torch.isfinite(y[1::3][:, :2]).all() and torch.isnan(y[1::3][:, 7]).all()
+
+
+@pytest.mark.parametrize("kind", ("f32", "bf16", "i8"))
+@pytest.mark.parametrize("sizes,n,k", (([3, 5], 40, 96), ([300, 200, 400], 900, 130), ([300, 200, 400], 900, 128), ([600], 32, 48)), ids=str)
+def test_grouped_without_any_row_of_x(sizes, n, k, kind):
+    """x_rows = 0: x is not looked at."""
+    e, rows = len(sizes), sum(sizes)
+    w, bias = torch.ones(e, n, k, device="cuda").to(T[kind]), torch.randn(e, n, device="cuda")
+    off, y = torch.tensor([0] + sizes).cumsum(0).to(torch.int32).cuda(), torch.zeros(rows, n, device="cuda")
+    call(capi.load().qcnn_op_grouped_matmul, capi.GroupedMatmul(y=ptr(y), w=ptr(w), offsets=ptr(off), bias=ptr(bias), ldx=k, ldy=n, ldw=k, w_stride=n * k,
+         rows=rows, experts=e, n=n, k=k, type=KIND[kind], out_type=capi.F32))
+    assert torch.equal(y, bias.repeat_interleave(torch.tensor(sizes, device="cuda"), 0))
