@@ -319,12 +319,13 @@ __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, un
                     *(T *)(at + row * (128 * TS) + (c ^ (row & 15)) * 16 + k * TS % 16) = v[i];
                 }
             }
-            const unsigned last = (unsigned)(a.k - 1) / (unsigned)a.group;  // (behind the last group x is zero)
+            const unsigned last = (unsigned)(a.k - 1) / (unsigned)a.group;
 #pragma unroll
             for (int j = 0; j < G::SI; ++j) {
                 const size_t e = (size_t)min(((unsigned)kb * 4 + set[j] * FL) / per, last) * a.n + nbase + col[j];
                 unsigned *sz = (unsigned *)(mine + NT * 1024 + j * 256) + lane;
                 *sz = S16 ? ((const uint16_t *)a.scale)[e] : ((const unsigned *)a.scale)[e];
+                if (kb * 128 + set[j] * (FL * 32) >= a.k) *sz = 0;  // behind the row's end x is zero: an infinite scale must not meet it
                 if (ZERO) sz[G::SI * 64] = ((const uint8_t *)a.zero)[e];
             }
         }

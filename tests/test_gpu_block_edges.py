@@ -1,11 +1,12 @@
 """GPU parity of the operators for blocks of language models at their borders.  Inputs, oracle and tolerances as in
 test_gpu_block_ops.py unless a test says otherwise."""
+import numpy as np
 import pytest
 import torch
 
 from oracle import np_blocks
 from qcnn_gpu_amd import capi
-from test_gpu_block_ops import KIND, T, call, close, np64, ptr
+from test_gpu_block_ops import KIND, T, call, close, np64, ptr, w4_run
 
 pytestmark = pytest.mark.gpu
 NAN, INF = float("nan"), float("inf")
@@ -71,3 +72,20 @@ def test_grouped_without_any_row_of_x(sizes, n, k, kind):
     call(capi.load().qcnn_op_grouped_matmul, capi.GroupedMatmul(y=ptr(y), w=ptr(w), offsets=ptr(off), bias=ptr(bias), ldx=k, ldy=n, ldw=k, w_stride=n * k,
          rows=rows, experts=e, n=n, k=k, type=KIND[kind], out_type=capi.F32))
     assert torch.equal(y, bias.repeat_interleave(torch.tensor(sizes, device="cuda"), 0))
+
+
+@pytest.mark.parametrize("kind", ("f32", "f16", "bf16"))
+@pytest.mark.parametrize("zeros", (False, True))
+@pytest.mark.parametrize("rows,k,group", ((1, 40, 32), (3, 33, 32), (2, 170, 64), (18, 330, 96), (40, 65, 64)))
+def test_w4_infinite_scale_of_the_last_group(rows, k, group, zeros, kind):
+    """The groups that a run of 128 k has behind the last one add nothing, also where the last one's scale is infinite."""
+    n, ng = 21, -(-k // group)
+    g = torch.Generator().manual_seed(k)
+    x = torch.randint(1, 4, (rows, k), generator=g).double()
+    codes = torch.randint(9, 16, (n, k + 1), generator=g, dtype=torch.uint8)
+    w = codes[:, 0:(k + 1) // 2 * 2:2] | codes[:, 1:(k + 1) // 2 * 2:2] << 4
+    scale = torch.ones(ng, n, dtype=torch.float64)
+    scale[-1, ::2], scale[-1, 1] = INF, -INF
+    zero = torch.full((ng, n), 7, dtype=torch.uint8) if zeros else None
+    y, want, _ = w4_run(x, w, scale, zero, None, group, kind, okind="f32")
+    assert np.array_equal(y.double().cpu().numpy(), want)
