@@ -375,7 +375,7 @@ typedef struct {
     const void *zero;  /* uint8 [ceil(k / group)][n], 0..15; NULL: 8 everywhere                           */
     const void *bias;  /* float [n] or NULL                                                               */
     size_t ldx, ldy, ldw;
-    int rows, n, k;    /* n <= 2^26, ldx <= 2^24, ldw <= 2^25                                             */
+    int rows, n, k;    /* n <= 2^26, ldx <= 2^24, ldw <= 2^25, ceil(rows / 16) * ceil(n / 16) <= 2^31     */
     int group;         /* a multiple of 32; the last group may be short                                   */
     int type, scale_type, out_type; /* QCNN_F32, QCNN_F16 or QCNN_BF16 each                               */
 } qcnn_matvec_w4_t;
@@ -402,7 +402,8 @@ typedef struct {
     const float *bias;        /* [experts][n] or NULL                                                     */
     const float *row_scale;   /* [rows] or NULL                                                           */
     size_t ldx, ldy, ldw, w_stride;
-    int rows, x_rows, experts, n, k;  /* experts <= 1024, n and k <= 2^28                                 */
+    int rows, x_rows, experts, n, k;  /* experts <= 1024, n and k <= 2^28,
+                                         (rows / 16 + min(rows, experts)) * ceil(n / 32) < 2^31           */
     int type;                 /* QCNN_F32, QCNN_F16, QCNN_BF16 or QCNN_I8                                 */
     int out_type;             /* QCNN_F32, QCNN_F16 or QCNN_BF16                                          */
     int act;                  /* QCNN_ACT_*                                                               */

@@ -61,6 +61,18 @@ __device__ __forceinline__ float block_act(float v, int act)
     return v;
 }
 
+// Workgroups of a launch, counted along x and y: a grid's width times the workgroup's threads has to stay below 2^32, so more
+// than 2^21 workgroups stand in rows of 2^21.  The last row may have some too many; they find nothing to do and leave.
+constexpr unsigned GRID_ROW = 1u << 21;
+__device__ __forceinline__ unsigned workgroup() { return blockIdx.y * GRID_ROW + blockIdx.x; }
+inline hipError_t grid_of(unsigned long long groups, dim3 &grid)
+{
+    const unsigned long long rows = (groups + GRID_ROW - 1) / GRID_ROW;
+    if (rows > 2047) return hipErrorNotSupported;  // workgroup() has 32 bits
+    grid = rows > 1 ? dim3(GRID_ROW, (unsigned)rows) : dim3((unsigned)groups);
+    return hipSuccess;
+}
+
 // Lets kernel `fn` have `bytes` of LDS beyond the 64 KB that need no asking; `asked` holds a bit for each device on which that has
 // been done (asking again at every launch is 0.5 us of the caller's time).
 inline hipError_t allow_lds(const void *fn, int bytes, std::atomic<unsigned long long> &asked)

@@ -136,7 +136,7 @@ struct Tiles {
 static hipError_t count_tiles(const qcnn_grouped_matmul_t &a, int TM, int TN, unsigned long long &tiles)
 {
     tiles = ((unsigned long long)(a.rows / TM) + (a.experts < a.rows ? a.experts : a.rows)) * ((a.n + TN - 1) / TN);
-    return tiles < 1ull << 31 ? hipSuccess : hipErrorInvalidConfiguration;
+    return tiles < 1ull << 31 ? hipSuccess : hipErrorNotSupported;
 }
 
 // N neighbouring outputs of one row.  `least` is 0 for ReLU, else -inf (a NaN passes either way).  STREAM: past the caches.
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(64 * KW *NW) void k_grouped_rows(const qcnn_grouped
     Tiles<16 * MT, 16 * NW> tiles;
     tiles.count(a);
     Tile t{0, 0, 0, 0, 1};
-    if (!tiles.get(a, blockIdx.x >> 3, t)) return;
+    if (!tiles.get(a, workgroup() >> 3, t)) return;
 
     // this lane's rows: one of w and, for each operand of x that this wave brings, one of x
     const int bytes = a.k * (int)sizeof(T), all = (bytes + RB - 1) / RB, turns = (all + KW - 1) / KW;
@@ -652,12 +652,14 @@ static hipError_t run_rows(const qcnn_grouped_matmul_t &a, bool al, hipStream_t 
     hipError_t e = count_tiles(a, 16 * MT, 16 * NW, tiles);
     if (e != hipSuccess) return e;
     const unsigned long long blocks = (tiles + 7) / 8 * 8;  // as many on each XCD
-    if (blocks * (64 * KW * NW) > 0xffffffffull) return hipErrorInvalidConfiguration;
+    dim3 grid;
+    e = grid_of(blocks, grid);
+    if (e != hipSuccess) return e;
     static std::atomic<unsigned long long> asked[2] = {{0}, {0}};
     const auto fn = al ? k_grouped_rows<T, MT, RB, KW, NW, KB, true> : k_grouped_rows<T, MT, RB, KW, NW, KB, false>;
     e = allow_lds((const void *)fn, G::LDS, asked[al]);
     if (e != hipSuccess) return e;
-    fn<<<(unsigned)blocks, 64 * KW * NW, G::LDS, s>>>(a);
+    fn<<<grid, 64 * KW * NW, G::LDS, s>>>(a);
     return hipGetLastError();
 }
 
@@ -707,7 +709,7 @@ __global__ __launch_bounds__(256) void k_grouped_narrow(const qcnn_grouped_matmu
     Tiles<TM, 64> tiles;
     tiles.count(a);
     Tile t{0, 0, 0, 0, 1};
-    if (!tiles.get(a, blockIdx.x >> 3, t)) return;
+    if (!tiles.get(a, workgroup() >> 3, t)) return;
 
     const int bytes = a.k * (int)sizeof(T);
     const bool pairs = a.out_type != QCNN_F32;
@@ -779,11 +781,12 @@ template <typename T, int NT, int OPS, int TM>
 static hipError_t launch_narrow(const qcnn_grouped_matmul_t &a, hipStream_t s)
 {
     unsigned long long tiles;
-    const hipError_t e = count_tiles(a, TM, 64, tiles);
+    hipError_t e = count_tiles(a, TM, 64, tiles);
     if (e != hipSuccess) return e;
-    const unsigned long long blocks = (tiles + 7) / 8 * 8;
-    if (blocks * 256 > 0xffffffffull) return hipErrorInvalidConfiguration;
-    k_grouped_narrow<T, NT, OPS, TM><<<(unsigned)blocks, 256, 0, s>>>(a);
+    dim3 grid;
+    e = grid_of((tiles + 7) / 8 * 8, grid);
+    if (e != hipSuccess) return e;
+    k_grouped_narrow<T, NT, OPS, TM><<<grid, 256, 0, s>>>(a);
     return hipGetLastError();
 }
 

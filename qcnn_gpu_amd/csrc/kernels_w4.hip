@@ -207,7 +207,9 @@ __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, un
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
     const int kq = wave / NW, nq = wave % NW;
-    const int n0 = ((int)(blockIdx.x % nblocks) * NW + nq) * 16 * NT, m0 = (int)(blockIdx.x / nblocks) * XROWS;
+    const unsigned at_n = workgroup() % nblocks, at_m = workgroup() / nblocks * XROWS;
+    if (at_m >= (unsigned)a.rows) return;
+    const int n0 = ((int)at_n * NW + nq) * 16 * NT, m0 = (int)at_m;
     const int rows = min(XROWS, a.rows - m0), row_bytes = (a.k + 1) >> 1;
 
     // runs of this k group: pairs, as two runs share the cache lines of the weight rows; the last run of all may be cut by
@@ -444,7 +446,7 @@ __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, un
 #pragma unroll
             for (int q = 0; q < 4; ++q) sums[kq * (OUT * 16 * MT) + (m * 16 + 4 * g + q) * OUT + nq * (16 * NT) + t * 16 + c16] = acc[t][m][q];
     __syncthreads();
-    const int base = (int)(blockIdx.x % nblocks) * OUT;
+    const int base = (int)at_n * OUT;
     for (int o = threadIdx.x; o < OUT * rows; o += 64 * KW * NW) {
         const int row = o / OUT, j = base + o % OUT;
         if (j >= a.n) continue;
@@ -462,12 +464,14 @@ static hipError_t launch(const qcnn_matvec_w4_t &a, hipStream_t s)
     typedef W4<T, NT, XROWS, FL, S16, ZERO, KW, NW, KB> G;
     const unsigned nblocks = (unsigned)((a.n + 16 * NT * NW - 1) / (16 * NT * NW));
     const unsigned long long blocks = (unsigned long long)nblocks * (((unsigned)a.rows + XROWS - 1) / XROWS);
-    if (blocks * (64 * G::WAVES) > 0xffffffffull) return hipErrorInvalidConfiguration;
+    dim3 grid;
+    hipError_t e = grid_of(blocks, grid);
+    if (e != hipSuccess) return e;
     const auto fn = k_w4<T, NT, XROWS, FL, S16, ZERO, KW, NW, KB>;
     static std::atomic<unsigned long long> asked{0};
-    const hipError_t e = allow_lds((const void *)fn, G::LDS, asked);
+    e = allow_lds((const void *)fn, G::LDS, asked);
     if (e != hipSuccess) return e;
-    fn<<<(unsigned)blocks, 64 * G::WAVES, G::LDS, s>>>(a, nblocks);
+    fn<<<grid, 64 * G::WAVES, G::LDS, s>>>(a, nblocks);
     return hipGetLastError();
 }
 

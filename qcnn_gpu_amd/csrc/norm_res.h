@@ -137,8 +137,8 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void k_norm_res(const qcnn_n
     __shared__ float red[LPR > 64 ? 2 * (LPR / 64) : 1];
     int turn = 0;
     const int t = threadIdx.x % LPR;
-    const size_t r = (size_t)blockIdx.x * RPB + threadIdx.x / LPR;
-    if (RPB > 1 && r >= (size_t)a.rows) return;  // whole rows leave (LPR <= 64: no barrier follows)
+    const size_t r = (size_t)workgroup() * RPB + threadIdx.x / LPR;
+    if (r >= (size_t)a.rows) return;  // whole rows leave, and where barriers follow (LPR > 64) whole workgroups
     const int d = a.d;
     const float inv_d = 1.f / (float)d;
     float v[CPT][VE];
@@ -275,11 +275,13 @@ static hipError_t run(const qcnn_norm_res_t &a, hipStream_t s)
     // the caches (256 x 4096 and two readers 11.6, 12.0 past them).
     const bool stream = (size_t)a.rows * a.d * sizeof(T) * ((a.h != nullptr) + (a.n != nullptr)) >= (size_t)8 << 20;
     const unsigned long long blocks = ((unsigned long long)a.rows + RPB - 1) / RPB;
-    if (blocks * BLOCK > 0xffffffffull) return hipErrorInvalidConfiguration;
+    dim3 grid;
+    const hipError_t e = grid_of(blocks, grid);
+    if (e != hipSuccess) return e;
     if (stream)
-        k_norm_res<T, LPR, CPT, true><<<(unsigned)blocks, BLOCK, 0, s>>>(a);
+        k_norm_res<T, LPR, CPT, true><<<grid, BLOCK, 0, s>>>(a);
     else
-        k_norm_res<T, LPR, CPT, false><<<(unsigned)blocks, BLOCK, 0, s>>>(a);
+        k_norm_res<T, LPR, CPT, false><<<grid, BLOCK, 0, s>>>(a);
     return hipGetLastError();
 }
 

@@ -89,3 +89,36 @@ def test_w4_infinite_scale_of_the_last_group(rows, k, group, zeros, kind):
     zero = torch.full((ng, n), 7, dtype=torch.uint8) if zeros else None
     y, want, _ = w4_run(x, w, scale, zero, None, group, kind, okind="f32")
     assert np.array_equal(y.double().cpu().numpy(), want)
+
+
+# ---- more workgroups than a row of a grid takes ----------------------------------------------------------
+def test_w4_rows_beyond_one_row_of_the_grid():
+    """2^28 rows make 2^23 workgroups of 512 threads."""
+    rows, n = (1 << 28) + 77, 1
+    x = torch.randint(-8, 9, (rows, 1), generator=torch.Generator("cuda").manual_seed(5), device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    y = torch.full((rows + 64, n), 77.0, dtype=torch.bfloat16, device="cuda")
+    w, s = torch.full((1, 1), 13, dtype=torch.uint8, device="cuda"), torch.full((1, 1), 0.5, device="cuda")
+    call(capi.load().qcnn_op_matvec_w4, capi.MatvecW4(x=ptr(x), y=ptr(y), w=ptr(w), scale=ptr(s), ldx=1, ldy=1, ldw=1, rows=rows, n=n, k=1, group=32,
+         type=capi.BF16, scale_type=capi.F32, out_type=capi.BF16))
+    assert torch.equal(y[:rows], x * 2.5) and (y[rows:] == 77).all()
+
+
+def test_norm_rows_beyond_one_row_of_the_grid():
+    """2^29 rows of one value make 2^24 workgroups of 256 threads."""
+    rows = (1 << 29) + 77
+    x = torch.randint(-8, 9, (rows,), generator=torch.Generator("cuda").manual_seed(6), device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    h = torch.full((rows + 64,), 77.0, dtype=torch.bfloat16, device="cuda")
+    call(capi.load().qcnn_op_norm_res, capi.NormRes(x=ptr(x), h=ptr(h), ldx=1, ldh=1, rows=rows, d=1, parts=1, type=capi.BF16, w_type=capi.F32, beta=0.5))
+    assert torch.equal(h[:rows], x * 0.5) and (h[rows:] == 77).all()
+
+
+def test_grouped_tiles_beyond_one_row_of_the_grid():
+    """One row for each of 32 experts with 2^25 outputs: 2^24 and more workgroups of 256 threads."""
+    e, n = 32, 1 << 25
+    g = torch.Generator("cuda").manual_seed(7)
+    w = torch.randint(-8, 9, (e, n), generator=g, device="cuda", dtype=torch.int8)
+    x = torch.arange(1, e + 1, device="cuda", dtype=torch.int8).view(e, 1)
+    y, off = torch.full((e + 1, n), 77.0, dtype=torch.float16, device="cuda"), torch.arange(e + 1, dtype=torch.int32, device="cuda")
+    call(capi.load().qcnn_op_grouped_matmul, capi.GroupedMatmul(x=ptr(x), y=ptr(y), w=ptr(w), offsets=ptr(off), ldx=1, ldy=n, ldw=1, w_stride=n, rows=e, x_rows=e,
+         experts=e, n=n, k=1, type=capi.I8, out_type=capi.F16))
+    assert torch.equal(y[:e], w.half() * x.half()) and (y[e:] == 77).all()
