@@ -375,7 +375,7 @@ typedef struct {
     const void *zero;  /* uint8 [ceil(k / group)][n], 0..15; NULL: 8 everywhere                           */
     const void *bias;  /* float [n] or NULL                                                               */
     size_t ldx, ldy, ldw;
-    int rows, n, k;    /* n <= 2^26, ldx <= 2^24, ldw <= 2^25, ceil(rows / 16) * ceil(n / 16) <= 2^31     */
+    int rows, n, k;    /* n <= 2^26, ldx <= 2^24, ldw <= 2^25                                             */
     int group;         /* a multiple of 32; the last group may be short                                   */
     int type, scale_type, out_type; /* QCNN_F32, QCNN_F16 or QCNN_BF16 each                               */
 } qcnn_matvec_w4_t;

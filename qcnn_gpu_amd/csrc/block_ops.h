@@ -61,8 +61,8 @@ __device__ __forceinline__ float block_act(float v, int act)
     return v;
 }
 
-// Workgroups of a launch, counted along x and y: a grid's width times the workgroup's threads has to stay below 2^32, so more
-// than 2^21 workgroups stand in rows of 2^21.  The last row may have some too many; they find nothing to do and leave.
+// Workgroups of a launch whose kernel finds its work by itself, counted along x and y: a grid's width times the workgroup's threads
+// has to stay below 2^32, so more than 2^21 workgroups stand in rows of 2^21; those too many in the last row find nothing.
 constexpr unsigned GRID_ROW = 1u << 21;
 __device__ __forceinline__ unsigned workgroup() { return blockIdx.y * GRID_ROW + blockIdx.x; }
 inline hipError_t grid_of(unsigned long long groups, dim3 &grid)

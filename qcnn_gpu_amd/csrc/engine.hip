@@ -1638,8 +1638,6 @@ int qcnn_op_matvec_w4(const qcnn_matvec_w4_t *a, void *stream)
     if (a->ldx < (size_t)a->k || a->ldy < (size_t)a->n || a->ldw < ((size_t)a->k + 1) / 2)
         return fail(QCNN_E_ARG, "row strides %zu, %zu, %zu are shorter than a row", a->ldx, a->ldy, a->ldw);
     if (too_far(a->ldx, a->rows) || too_far(a->ldy, a->rows) || too_far(a->ldw, a->n)) return fail(QCNN_E_ARG, "row strides too large");
-    if (((size_t)a->rows + 15) / 16 * (((size_t)a->n + 15) / 16) > (size_t)1 << 31)
-        return fail(QCNN_E_UNSUPPORTED, "%d rows and %d outputs: more than 2^31 tiles of 16 x 16", a->rows, a->n);
     if (a->rows == 0) return QCNN_OK;
     if (!a->x || !a->y || !a->w || !a->scale) return fail(QCNN_E_ARG, "null pointer");
     if (!aligned(a->x, type_size(a->type)) || !aligned(a->y, type_size(a->out_type)) || !aligned(a->scale, type_size(a->scale_type)) ||

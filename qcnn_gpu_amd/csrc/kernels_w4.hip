@@ -207,9 +207,7 @@ __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, un
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, g = lane >> 4;
     const int kq = wave / NW, nq = wave % NW;
-    const unsigned at_n = workgroup() % nblocks, at_m = workgroup() / nblocks * XROWS;
-    if (at_m >= (unsigned)a.rows) return;
-    const int n0 = ((int)at_n * NW + nq) * 16 * NT, m0 = (int)at_m;
+    const int n0 = ((int)(blockIdx.x % nblocks) * NW + nq) * 16 * NT, m0 = (int)(blockIdx.x / nblocks) * XROWS;
     const int rows = min(XROWS, a.rows - m0), row_bytes = (a.k + 1) >> 1;
 
     // runs of this k group: pairs, as two runs share the cache lines of the weight rows; the last run of all may be cut by
@@ -446,7 +444,7 @@ __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, un
 #pragma unroll
             for (int q = 0; q < 4; ++q) sums[kq * (OUT * 16 * MT) + (m * 16 + 4 * g + q) * OUT + nq * (16 * NT) + t * 16 + c16] = acc[t][m][q];
     __syncthreads();
-    const int base = (int)at_n * OUT;
+    const int base = (int)(blockIdx.x % nblocks) * OUT;
     for (int o = threadIdx.x; o < OUT * rows; o += 64 * KW * NW) {
         const int row = o / OUT, j = base + o % OUT;
         if (j >= a.n) continue;
@@ -463,16 +461,23 @@ static hipError_t launch(const qcnn_matvec_w4_t &a, hipStream_t s)
 {
     typedef W4<T, NT, XROWS, FL, S16, ZERO, KW, NW, KB> G;
     const unsigned nblocks = (unsigned)((a.n + 16 * NT * NW - 1) / (16 * NT * NW));
-    const unsigned long long blocks = (unsigned long long)nblocks * (((unsigned)a.rows + XROWS - 1) / XROWS);
-    dim3 grid;
-    hipError_t e = grid_of(blocks, grid);
-    if (e != hipSuccess) return e;
     const auto fn = k_w4<T, NT, XROWS, FL, S16, ZERO, KW, NW, KB>;
     static std::atomic<unsigned long long> asked{0};
-    e = allow_lds((const void *)fn, G::LDS, asked);
+    const hipError_t e = allow_lds((const void *)fn, G::LDS, asked);
     if (e != hipSuccess) return e;
-    fn<<<grid, 64 * G::WAVES, G::LDS, s>>>(a, nblocks);
-    return hipGetLastError();
+    // a launch's threads have to stay below 2^32: more rows take several (n <= 2^26: at least XROWS rows fit)
+    const unsigned most = 0xffffffffu / (64 * G::WAVES) / nblocks;
+    if (!most) return hipErrorNotSupported;
+    qcnn_matvec_w4_t part = a;
+    for (long long done = 0; done < a.rows; done += (long long)most * XROWS) {
+        part.rows = (int)(a.rows - done < (long long)most * XROWS ? a.rows - done : (long long)most * XROWS);
+        part.x = (const char *)a.x + (size_t)done * a.ldx * sizeof(T);
+        part.y = (char *)a.y + (size_t)done * a.ldy * (a.out_type == QCNN_F32 ? 4 : 2);
+        fn<<<nblocks * (((unsigned)part.rows + XROWS - 1) / XROWS), 64 * G::WAVES, G::LDS, s>>>(part, nblocks);
+        const hipError_t launched = hipGetLastError();
+        if (launched != hipSuccess) return launched;
+    }
+    return hipSuccess;
 }
 
 template <typename T, int NT, int XROWS, int FL, int KW, int NW, int KB>

@@ -137,8 +137,8 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void k_norm_res(const qcnn_n
     __shared__ float red[LPR > 64 ? 2 * (LPR / 64) : 1];
     int turn = 0;
     const int t = threadIdx.x % LPR;
-    const size_t r = (size_t)workgroup() * RPB + threadIdx.x / LPR;
-    if (r >= (size_t)a.rows) return;  // whole rows leave, and where barriers follow (LPR > 64) whole workgroups
+    const size_t r = (size_t)blockIdx.x * RPB + threadIdx.x / LPR;
+    if (RPB > 1 && r >= (size_t)a.rows) return;  // whole rows leave (LPR <= 64: no barrier follows)
     const int d = a.d;
     const float inv_d = 1.f / (float)d;
     float v[CPT][VE];
@@ -274,15 +274,29 @@ static hipError_t run(const qcnn_norm_res_t &a, hipStream_t s)
     // takes as long either way (4096 x 1024 and two readers 18.8 -> 17.8, 16384 x 4096 207 -> 206), but finds smaller ones sooner in
     // the caches (256 x 4096 and two readers 11.6, 12.0 past them).
     const bool stream = (size_t)a.rows * a.d * sizeof(T) * ((a.h != nullptr) + (a.n != nullptr)) >= (size_t)8 << 20;
-    const unsigned long long blocks = ((unsigned long long)a.rows + RPB - 1) / RPB;
-    dim3 grid;
-    const hipError_t e = grid_of(blocks, grid);
-    if (e != hipSuccess) return e;
-    if (stream)
-        k_norm_res<T, LPR, CPT, true><<<grid, BLOCK, 0, s>>>(a);
-    else
-        k_norm_res<T, LPR, CPT, false><<<grid, BLOCK, 0, s>>>(a);
-    return hipGetLastError();
+    // A launch's threads have to stay below 2^32: more rows take several, that part where a row of gate does, or inside one.
+    const long long most = (0xffffffffu / BLOCK) * (long long)RPB, gate_rows = a.gate ? a.gate_rows : 1;
+    qcnn_norm_res_t part = a;
+    for (long long done = 0; done < a.rows; done += part.rows) {
+        const long long fit = gate_rows <= most ? most / gate_rows * gate_rows : gate_rows - done % gate_rows < most ? gate_rows - done % gate_rows : most;
+        part.rows = (int)(a.rows - done < fit ? a.rows - done : fit);
+        part.x = (const T *)a.x + (size_t)done * a.ldx;
+        if (a.index)
+            part.index = a.index + (size_t)done * a.parts;
+        else if (a.y)
+            part.y = (const T *)a.y + (size_t)done * a.ldy;
+        if (a.gate) part.gate = (const T *)a.gate + (size_t)(done / gate_rows) * a.ldg;
+        if (a.h) part.h = (T *)a.h + (size_t)done * a.ldh;
+        if (a.n) part.n = (T *)a.n + (size_t)done * a.ldn;
+        const unsigned blocks = ((unsigned)part.rows + RPB - 1) / RPB;
+        if (stream)
+            k_norm_res<T, LPR, CPT, true><<<blocks, BLOCK, 0, s>>>(part);
+        else
+            k_norm_res<T, LPR, CPT, false><<<blocks, BLOCK, 0, s>>>(part);
+        const hipError_t launched = hipGetLastError();
+        if (launched != hipSuccess) return launched;
+    }
+    return hipSuccess;
 }
 
 // Threads a row and chunks a thread.  A row of at most 64 chunks fits one wave (no barrier).  With up to 512 rows the time is one

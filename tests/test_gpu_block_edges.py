@@ -91,8 +91,8 @@ def test_w4_infinite_scale_of_the_last_group(rows, k, group, zeros, kind):
     assert np.array_equal(y.double().cpu().numpy(), want)
 
 
-# ---- more workgroups than a row of a grid takes ----------------------------------------------------------
-def test_w4_rows_beyond_one_row_of_the_grid():
+# ---- more workgroups than a launch, or a row of its grid, takes --------------------------------------------
+def test_w4_rows_beyond_one_launch():
     """2^28 rows make 2^23 workgroups of 512 threads."""
     rows, n = (1 << 28) + 77, 1
     x = torch.randint(-8, 9, (rows, 1), generator=torch.Generator("cuda").manual_seed(5), device="cuda", dtype=torch.int8).to(torch.bfloat16)
@@ -103,7 +103,7 @@ def test_w4_rows_beyond_one_row_of_the_grid():
     assert torch.equal(y[:rows], x * 2.5) and (y[rows:] == 77).all()
 
 
-def test_norm_rows_beyond_one_row_of_the_grid():
+def test_norm_rows_beyond_one_launch():
     """2^29 rows of one value make 2^24 workgroups of 256 threads."""
     rows = (1 << 29) + 77
     x = torch.randint(-8, 9, (rows,), generator=torch.Generator("cuda").manual_seed(6), device="cuda", dtype=torch.int8).to(torch.bfloat16)
@@ -112,7 +112,26 @@ def test_norm_rows_beyond_one_row_of_the_grid():
     assert torch.equal(h[:rows], x * 0.5) and (h[rows:] == 77).all()
 
 
-def test_grouped_tiles_beyond_one_row_of_the_grid():
+@pytest.mark.parametrize("gate_rows", (7, (1 << 29) - 5, 1 << 30))
+def test_norm_gates_and_indices_beyond_one_launch(gate_rows):
+    """A launch takes 2^29 - 32 rows of one value: rows of gate that end before its end, behind it and never."""
+    rows = (1 << 29) + 77
+    g = torch.Generator("cuda").manual_seed(gate_rows)
+    x, y = (torch.randint(-8, 9, (rows,), generator=g, device="cuda", dtype=torch.int8).to(torch.bfloat16) for _ in range(2))
+    gate = torch.randint(-4, 5, (-(-rows // gate_rows),), generator=g, device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    index = torch.arange(rows - 1, -1, -1, device="cuda", dtype=torch.int32)
+    n = torch.empty_like(x)
+    want = x + y.flip(0) * gate.repeat_interleave(gate_rows)[:rows]
+    call(capi.load().qcnn_op_norm_res, capi.NormRes(x=ptr(x), y=ptr(y), index=ptr(index), gate=ptr(gate), h=ptr(x), n=ptr(n), ldx=1, ldy=1, ldg=1, ldh=1, ldn=1, rows=rows,
+         y_rows=rows, d=1, parts=1, gate_rows=gate_rows, type=capi.BF16, w_type=capi.F32, alpha=1.0, beta=1.0))
+    assert torch.equal(x, want) and torch.equal(n, want)
+    y0 = y.clone()
+    call(capi.load().qcnn_op_norm_res, capi.NormRes(x=ptr(x), y=ptr(y), h=ptr(y), n=ptr(n), ldx=1, ldy=1, ldh=1, ldn=1, rows=rows, y_rows=rows, d=1, parts=1,
+         type=capi.BF16, w_type=capi.F32, alpha=1.0, beta=0.0, pre=capi.NORM_LAYER, pre_eps=1.0))
+    assert torch.equal(y, y0) and (n == 0).all()
+
+
+def test_grouped_tiles_beyond_one_launch():
     """One row for each of 32 experts with 2^25 outputs: 2^24 and more workgroups of 256 threads."""
     e, n = 32, 1 << 25
     g = torch.Generator("cuda").manual_seed(7)
