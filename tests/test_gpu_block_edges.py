@@ -141,3 +141,87 @@ def test_grouped_tiles_beyond_one_launch():
     call(capi.load().qcnn_op_grouped_matmul, capi.GroupedMatmul(x=ptr(x), y=ptr(y), w=ptr(w), offsets=ptr(off), ldx=1, ldy=n, ldw=1, w_stride=n, rows=e, x_rows=e,
          experts=e, n=n, k=1, type=capi.I8, out_type=capi.F16))
     assert torch.equal(y[:e], w.half() * x.half()) and (y[e:] == 77).all()
+
+
+# ---- the loops of the tile kernels -----------------------------------------------------------------------
+def tile_of(sizes, n, k, kind, aligned=True):
+    """The launch rules of kernels_grouped.hip for calls that reach a tile kernel: its height and width (None: another kernel)."""
+    z = T[kind].itemsize
+    rows, e = sum(sizes), len(sizes)
+    avg = rows // e
+
+    def tiles(t):
+        return (rows // t + min(rows, e)) * -(-n // t)
+    if (n <= 64 and k * z <= 256 and avg >= 512) or tiles(32) < 128 or avg <= 24 or tiles(64) < (160 if z == 4 else 64):
+        return None
+    if tiles(128) < (1024 if z == 4 else 256):
+        return 64
+    if z < 4 and aligned and k * z % 16 == 0 and avg >= 256 and tiles(256) >= (240 if k >= 2048 else 512):
+        return 256
+    return 128
+
+
+def tile_run(sizes, n, k, kind, seed, gather):
+    """Small whole numbers, sums below 2^24: every kernel's result is exact and equal to the product in 64 bits."""
+    g = torch.Generator("cuda").manual_seed(seed)
+    e, rows = len(sizes), sum(sizes)
+    whole = lambda *s: torch.randint(-3, 4, s, generator=g, device="cuda", dtype=torch.int8)  # noqa: E731
+    xrows = rows // 2 if gather else rows
+    x, w = whole(xrows, k), whole(e, n, k)
+    src = torch.randint(0, xrows, (rows,), generator=g, device="cuda", dtype=torch.int32) if gather else None
+    xt, wt = x.to(T[kind]), w.to(T[kind])
+    off = torch.tensor([0] + sizes).cumsum(0).to(torch.int32).cuda()
+    y = torch.full((rows + 5, n), 77.0, device="cuda")
+    call(capi.load().qcnn_op_grouped_matmul, capi.GroupedMatmul(x=ptr(xt), y=ptr(y), w=ptr(wt), offsets=ptr(off), src=ptr(src), ldx=k, ldy=n, ldw=k, w_stride=n * k,
+         rows=rows, x_rows=xrows, experts=e, n=n, k=k, type=KIND[kind], out_type=capi.F32))
+    at = 0
+    for i, c in enumerate(sizes):
+        if c:
+            v = x[src[at:at + c].long()] if gather else x[at:at + c]
+            assert torch.equal(y[at:at + c].double(), v.double() @ w[i].double().t()), (i, kind, n, k)
+        at += c
+    assert (y[rows:] == 77).all()
+
+
+# by float32 rows and tile: rows of the experts, outputs; and bytes of k: fewer steps of 64 than the loop begins with, the loop once, its end with one and two steps over, an unfinished step
+LOADS = {(False, 64): ([150, 0, 33, 260, 64], 420), (False, 128): ([700, 129, 0, 1200, 64, 128], 2100), (False, 256): ([3000, 257, 1, 4200, 0, 900, 128], 4100),
+         (True, 64): ([150, 0, 33, 260, 64], 1000), (True, 128): ([3000, 129, 0, 3100, 64, 128], 2450)}
+STEPS = (64, 320, 384, 448, 512, 528, 1024, 1040)
+
+
+@pytest.mark.parametrize("kind", ("f32", "f16", "bf16", "i8"))
+@pytest.mark.parametrize("tile", (64, 128, 256))
+@pytest.mark.parametrize("gather", (False, True))
+def test_grouped_tile_loops(tile, kind, gather):
+    """Every length of the loop over k in every tile kernel; loads that leave short tiles, halves, and several tiles to a workgroup."""
+    if tile == 256 and kind == "f32":
+        assert tile_of([9000], 9000, 512, kind) == 128  # float32 has no such tiles
+        return
+    sizes, n = LOADS[kind == "f32", tile]
+    z = T[kind].itemsize
+    for i, bytes_ in enumerate(STEPS):
+        k = bytes_ // z
+        assert tile_of(sizes, n, k, kind) == tile, (k, tile_of(sizes, n, k, kind))
+        tile_run(sizes, n, k, kind, 10 * tile + i, gather)
+
+
+@pytest.mark.parametrize("kind", ("f16", "bf16", "i8"))
+def test_grouped_large_tiles_by_long_k(kind):
+    """240 tiles are enough for 256 x 256 from k = 2048 on; below, 128 x 128."""
+    sizes, n = [1000, 2000, 300, 700], 3100
+    assert [tile_of(sizes, n, k, kind) for k in (2032, 2048, 2080)] == [128, 256, 256]
+    for k in (2032, 2048, 2080):
+        tile_run(sizes, n, k, kind, k, False)
+
+
+@pytest.mark.parametrize("kind", ("f32", "f16", "bf16", "i8"))
+def test_grouped_tile_loops_of_unaligned_rows(kind):
+    """Rows that are no whole chunks go through registers: 64 x 64 and 128 x 128 tiles alone."""
+    z = T[kind].itemsize
+    for tile in (64, 128):
+        sizes, n = LOADS[kind == "f32", tile]
+        for k in (1, 63 // z, 64 // z + 1, 130 // z + 1, 200 // z + 1, 600 // z + 1):
+            if k * z % 16 == 0:
+                k += 1
+            assert tile_of(sizes, n, k, kind) == tile
+            tile_run(sizes, n, k, kind, 7 * k, k % 2 == 0)
