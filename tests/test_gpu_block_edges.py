@@ -6,7 +6,7 @@ import torch
 
 from oracle import np_blocks
 from qcnn_gpu_amd import capi
-from test_gpu_block_ops import KIND, T, call, close, np64, ptr, w4_run
+from test_gpu_block_ops import KIND, T, call, close, grouped_run, np64, ptr, w4_run
 
 pytestmark = pytest.mark.gpu
 NAN, INF = float("nan"), float("inf")
@@ -225,3 +225,50 @@ def test_grouped_tile_loops_of_unaligned_rows(kind):
                 k += 1
             assert tile_of(sizes, n, k, kind) == tile
             tile_run(sizes, n, k, kind, 7 * k, k % 2 == 0)
+
+
+# ---- the size of the rounding error at a model's row lengths ---------------------------------------------
+# The bound that holds for every input grows with k times the sum of the magnitudes, far above what random inputs show.  These
+# tests look at the root mean square over the outputs.  An addition in float32 is off by at most U of its result, U / sqrt(3) at
+# most in the mean; of N additions in a row of terms of rms t the j-th result is about sqrt(j) t, so that the sum is off by
+# U t sqrt(sum j / 3) <= U sqrt(N / 6) * (sqrt(N) t): U sqrt(N / 6) times the L2 norm of the terms.  Other orders of the sum have
+# shorter chains.  Twice that is allowed, and one rounding of the result.
+U = np_blocks.U
+
+
+def rms(v):
+    return float(np.sqrt(np.mean(np.square(v))))
+
+
+@pytest.mark.parametrize("kind", ("f32", "f16", "bf16"))
+@pytest.mark.parametrize("rows,n,k,group", ((1, 512, 4096, 128), (16, 300, 4096, 64), (48, 200, 8192, 32), (4, 400, 16384, 16384)))
+def test_w4_error_of_long_rows(rows, n, k, group, kind):
+    g = torch.Generator().manual_seed(k + rows)
+    x = torch.randn(rows, k, generator=g, dtype=torch.float64)
+    w = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8)
+    scale = (0.5 + torch.rand(k // group, n, generator=g, dtype=torch.float64)) / k ** 0.5
+    zero = torch.randint(0, 16, (k // group, n), generator=g, dtype=torch.uint8)
+    y, want, _ = w4_run(x, w, scale, zero, None, group, kind, skind="f32", okind="f32")
+    x = x.to(T[kind]).double().numpy()
+    q = np.stack((w.numpy() & 15, w.numpy() >> 4), -1).reshape(n, k).astype(np.float64)
+    s = np.repeat(scale.float().double().numpy(), group, 0).T
+    z = np.repeat(zero.numpy().astype(np.float64), group, 0).T
+
+    def l2(of):  # of the terms of each output
+        return np.sqrt(np.square(x) @ np.square(s * of).T)
+    add = -8.0 if kind == "f32" else 16.0  # what the codes are summed with, and what is taken off again
+    chain = group * (3 if kind == "f32" else 1)  # float32 rows: three parts of each value
+    tol = 2 * U * (np.sqrt(chain / 6) * np.hypot(l2(q + add), l2(z + add)) + np.sqrt(k / group / 6) * l2(q - z)) + U * np.abs(want) + 2 * U * l2(q + add)
+    assert rms(y.double().cpu().numpy() - want) <= rms(tol)
+
+
+@pytest.mark.parametrize("kind", ("f32", "f16", "bf16"))
+@pytest.mark.parametrize("sizes,n,k", (([2, 1, 0, 3], 300, 4096), ([20] * 8, 256, 8192), ([300, 200], 500, 4096), ([1200, 848], 1100, 2048)), ids=str)
+def test_grouped_error_of_long_rows(sizes, n, k, kind):
+    y, want, _ = grouped_run(sizes, n, k, kind, "f32", k + n)
+    g = torch.Generator().manual_seed(k + n)  # the inputs that grouped_run made
+    rows, e = sum(sizes), len(sizes)
+    x, w = torch.randn(rows, k, generator=g, dtype=torch.float64), torch.randn(e * n, k, generator=g, dtype=torch.float64) / k ** 0.5
+    x, w = (t.to(T[kind]).double().square() for t in (x, w.view(e, n, k)))
+    l2 = torch.cat([p @ v.t() for p, v in zip(x.split(sizes), w)]).sqrt().numpy()
+    assert rms(y.double().cpu().numpy() - want) <= rms(2 * U * np.sqrt(k / 6) * l2 + U * np.abs(want))
