@@ -1,4 +1,4 @@
-// Shared pieces of the operators for blocks of language models (kernels_w4.hip, kernels_grouped.hip, kernels_norm.hip).
+// Shared pieces of the operators for blocks of language models (kernels_w4.hip, kernels_grouped.hip, norm_res.h).
 #pragma once
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -13,6 +13,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+// 16 bytes at any address: global loads and stores of gfx950 take any, and 16 bytes that cross a cache line cost one line more.
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 struct bf16_t {
     uint16_t bits;
@@ -31,13 +35,7 @@ __device__ __forceinline__ void from_f32(float v, bf16_t &o)  // round to neares
     __builtin_memcpy(&o, &r, 2);
 }
 
-// One value of a type known at run time (uniform over the launch): scales, biases and the outputs of the products.
-__device__ __forceinline__ float load_typed(const void *p, size_t i, int type)
-{
-    if (type == QCNN_F32) return ((const float *)p)[i];
-    if (type == QCNN_F16) return (float)((const f16_t *)p)[i];
-    return to_f32(((const bf16_t *)p)[i]);
-}
+// One value into an output whose type is known at run time (uniform over the launch).
 __device__ __forceinline__ void store_typed(void *p, size_t i, int type, float v)
 {
     if (type == QCNN_F32) {
@@ -48,6 +46,30 @@ __device__ __forceinline__ void store_typed(void *p, size_t i, int type, float v
         bf16_t b;
         from_f32(v, b);
         ((bf16_t *)p)[i] = b;
+    }
+}
+
+// 16 x 16 outputs, 32 k: lane l holds k 8 (l >> 4) .. 8 (l >> 4) + 7 of row l & 15 of either operand.
+__device__ __forceinline__ f32x4 mma(f16_t, u32x4 a, u32x4 b, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(bf16_t, u32x4 a, u32x4 b, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Waits until at most min(runs, MOST) runs' loads, and nothing else, are on their way.
+template <int MOST, int LOADS>
+__device__ __forceinline__ void wait_for_all_but(int runs)
+{
+    if constexpr (MOST <= 0) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    } else {
+        if (runs >= MOST)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * MOST) : "memory");
+        else
+            wait_for_all_but<MOST - 1, LOADS>(runs);
     }
 }
 

@@ -6,8 +6,6 @@
 
 namespace qcnn {
 
-typedef u32x4 u32x4_any __attribute__((aligned(1)));  // global loads and stores take any address
-
 // 16 bytes of a row are a chunk; a matrix instruction of 16 x 16 outputs takes a chunk of every lane: lane l holds
 // chunk (l >> 4) of four of row l & 15.  Both operands come in the same order, so the order of k inside a chunk is free:
 // float32 takes four instructions, element i of every lane's chunk each.
@@ -21,17 +19,7 @@ struct Mma<int8_t> {
     typedef i32x4 acc_t;
     typedef int one_t;
 };
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-__device__ __forceinline__ f32x4 mma(f16_t, u32x4 a, u32x4 b, f32x4 c)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mma(bf16_t, u32x4 a, u32x4 b, f32x4 c)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
 __device__ __forceinline__ i32x4 mma(int8_t, u32x4 a, u32x4 b, i32x4 c)
 {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
@@ -483,20 +471,6 @@ struct RowsGeom {
     static constexpr int LDS = KW * R * RUN > SUMS ? KW * R * RUN : SUMS;
     static_assert(MT * OPS % NW == 0 && LOADS * (R - 2) < 64 && LDS <= 163840, "runs fit");
 };
-
-// Waits until at most min(runs, MOST) runs' loads, and nothing else, are on their way.
-template <int MOST, int LOADS>
-__device__ __forceinline__ void wait_for_all_but(int runs)
-{
-    if constexpr (MOST <= 0) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    } else {
-        if (runs >= MOST)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * MOST) : "memory");
-        else
-            wait_for_all_but<MOST - 1, LOADS>(runs);
-    }
-}
 
 template <typename T, int MT, int RB, int KW, int NW, int KB, bool ALIGNED>
 __global__ __launch_bounds__(64 * KW *NW) void k_grouped_rows(const qcnn_grouped_matmul_t a)

@@ -28,10 +28,6 @@
 
 namespace qcnn {
 
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef u32x4 u32x4_any __attribute__((aligned(1)));
-
 #pragma clang diagnostic ignored "-Winline-asm"  // m0 in the clobber lists of the direct loads
 
 // x as it is loaded (RAW registers of 4 for 8 values) and as the matrix instruction takes it (PARTS operands)
@@ -125,14 +121,6 @@ __device__ __forceinline__ u32x4 codes(unsigned w)
                  and_or(byte_times<2>(w, C::BY), C::MASK, C::MAGIC), and_or(byte_times<3>(w, C::BY), C::MASK, C::MAGIC)};
 }
 
-__device__ __forceinline__ f32x4 mma(f16_t, u32x4 x, u32x4 w, f32x4 c)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, w), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mma(bf16_t, u32x4 x, u32x4 w, f32x4 c)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, w), c, 0, 0, 0);
-}
 __device__ __forceinline__ f32x4 mma(float, u32x4 x, u32x4 w, f32x4 c) { return mma(bf16_t(), x, w, c); }
 
 // dwords j of lanes l, l + 16, l + 32, l + 48 change places: lane l + 16 i's dword j goes to lane l + 16 j's dword i
@@ -166,20 +154,6 @@ __device__ __forceinline__ const char *uniform(const char *p)
     const unsigned long long u = (unsigned long long)p;
     const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)u), hi = __builtin_amdgcn_readfirstlane((unsigned)(u >> 32));  // (it returns int)
     return (const char *)((unsigned long long)hi << 32 | lo);
-}
-
-// Waits until at most min(runs, MOST) runs' loads, and nothing else, are on their way.
-template <int MOST, int LOADS>
-__device__ __forceinline__ void wait_for_all_but(int runs)
-{
-    if constexpr (MOST <= 0) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    } else {
-        if (runs >= MOST)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * MOST) : "memory");
-        else
-            wait_for_all_but<MOST - 1, LOADS>(runs);
-    }
 }
 
 // LDS of one run of 128 k: x of XROWS rows for the NW waves, then for each wave its codes (1 KB a tile of 16 outputs) and

@@ -15,10 +15,7 @@
 
 namespace qcnn {
 
-// 16 bytes of a row as they stand in memory.  The address need not be aligned: global loads and stores of gfx950 take
-// any address, and a chunk that crosses a cache line costs one line more.
-typedef u32x4 u32x4_any __attribute__((aligned(1)));
-
+// 16 bytes of a row as they stand in memory.
 template <typename T>
 struct Chunk {
     static constexpr int VE = 16 / sizeof(T);
