@@ -366,7 +366,9 @@ enum {
  * for any number of rows (made for 1 to 64, where reading the weights is the cost; more rows run in passes of 16 to 64).
  * Sums are float32, the result is rounded once.  Half and bfloat16 rows are summed with 16 + q for q and the surplus is
  * taken off at the end of each group: in float32, beside the sum itself.  x must be finite, and 32 times the sum of a
- * row's |x| within float32's range: else NaN may come out. */
+ * row's |x| within float32's range: else NaN may come out.  With random codes and x that leaves errors of 1e-7 to 3e-7 (root mean
+ * square) of the L2 norm of an output's terms at k = 4096.  float32 rows are taken apart into bfloat16 parts: values below 2^-109
+ * lose their bits below 2^-133. */
 typedef struct {
     const void *x;     /* [rows][ldx] of `type`                                                           */
     void *y;           /* [rows][ldy] of `out_type`                                                       */

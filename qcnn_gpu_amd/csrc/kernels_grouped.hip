@@ -43,9 +43,9 @@ struct Tile {
 // run on an XCD at a time then share 8 row tiles of x and 4 column tiles of w.
 // The offsets are device memory, so each wave adds up the tiles itself, 64 experts at a time over its lanes.
 // PARTS = 2: a tile of at most half of its rows is made as a half, and where the last round of an XCD's workgroups, PER_CU
-// on a CU, would leave half of its CUs idle, its tiles are cut in halves (4096 rows over 8, 2048 x 4096 bfloat16 129 -> 123 us,
-// 16384 over 16, 4096 x 2048 336 -> 327, int8 8192 over 8, 4096 x 4096 198 -> 192; quarters, and halves of 64 x 64 tiles,
-// were no faster).
+// on a CU, would leave half of its CUs idle, its tiles are cut in halves (measured as the table at `pick`: 4096 rows over 8, 2048 x 4096
+// bfloat16 123 -> 116 us, 16384 over 16, 4096 x 2048 312 -> 308, int8 8192 over 8, 4096 x 4096 184 -> 174; quarters, and halves of
+// 64 x 64 tiles, were no faster).
 template <int TM, int TN, int PARTS = 1, int PER_CU = 1>
 struct Tiles {
     unsigned all, nt;  // row tiles of all experts, column tiles
@@ -250,9 +250,9 @@ __device__ __forceinline__ void load_to_lds(const char *from, unsigned lds)
 // of the 256 bytes that the banks hold.
 // ALIGNED (rows begin at multiples of 16 bytes and hold whole chunks): loads go straight to LDS, a lane whose row
 // has ended loads zeros.  Otherwise loads of any address go through registers, a step ahead of LDS.
-// Measured with tiles of 256 x 256, one expert: 8192 x 8192 x 8192 1214 TFLOP/s in bfloat16 and 2270 TOP/s in int8, where
-// the power limit holds the clock; 16 experts of 1024 rows, 4096 x 2048: 1040, the epilogues and the ragged last round take
-// the rest.
+// Measured with tiles of 256 x 256, one expert: 8192 x 8192 x 8192 1260 TFLOP/s in bfloat16 (the library's product 1330 to 1375)
+// and 2280 TOP/s in int8; 16384 rows over 16, 4096 x 2048: 300 to 308 us, 890 to 916 TFLOP/s: short last tiles, the last round and the
+// hand-over between tiles, a chain of waits, take the rest.
 template <int TM, int TN, int WM, int WN>
 struct TileGeom {
     static constexpr int LDS = 4 * (TM + TN) * 64, PER_CU = 163840 / LDS < 8 / (WM * WN) ? 163840 / LDS : 8 / (WM * WN);
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void k_grouped_tile(const qcnn_grou
 // KW x NW, NW share out the outputs and KW the k, in runs of RB bytes, and the KW sums meet in LDS at the end.  Direct loads
 // bring the chunks in the order of the matrix instruction's lanes, R - 1 runs ahead: 1 KB of LDS is one operand, 64 bytes of
 // k of 16 rows.  x is shared by the NW waves of a k group (one barrier a run, none for NW = 1), and of sixteen rows
-// only those that there are ask for it.  64 rows of 64 experts, 1024 x 2048 bfloat16: 34 to 40 us, 4.1 to 4.8 TB/s.
+// only those that there are ask for it.  64 rows of 64 experts, 1024 x 2048 bfloat16, cold: 38 to 40 us, 4.1 to 4.3 TB/s.
 template <typename T, int MT, int RB, int KW, int NW, int KB>
 struct RowsGeom {
     static constexpr int OPS = RB / 64, WAVES = KW * NW;
@@ -673,7 +673,8 @@ static hipError_t run_tile(const qcnn_grouped_matmul_t &a, bool al, hipStream_t 
 // A wave keeps the weights of all outputs in registers and runs over its rows, four tiles of sixteen at a time, straight
 // from memory into matrix instructions.  Outputs of two bytes stand in the tiles as output_at has them, so that a lane
 // has 16 bytes of a row either way and four lanes write 64 side by side, past the caches, which the output would only
-// wash out (798720 rows, 48 int8 to 32 float32: 33.6 us, 46.6 through them).
+// wash out (798720 rows, 48 int8 to 32 float32: 33.4 us where the last cache holds x, 46.6 through them; with cold x 53, and
+// 46.6 through them).
 template <typename T, int NT, int OPS, int TM>
 __global__ __launch_bounds__(256) void k_grouped_narrow(const qcnn_grouped_matmul_t a)
 {
@@ -764,7 +765,7 @@ static hipError_t launch_narrow(const qcnn_grouped_matmul_t &a, hipStream_t s)
     return hipGetLastError();
 }
 
-// 512 rows a workgroup where that makes enough of them, else 64 (3968 rows of 209 bytes 28 -> 9 us).
+// 512 rows a workgroup where that makes enough of them, else 64 (3968 rows of 209 bytes 25 -> 9.8 us).
 template <typename T, int NT, int OPS>
 static hipError_t run_narrow(const qcnn_grouped_matmul_t &a, hipStream_t s)
 {
@@ -779,18 +780,22 @@ static hipError_t pick(qcnn_grouped_matmul_t a, hipStream_t s)
     const bool al = (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.w % 16 == 0 && a.ldx * z % 16 == 0 && a.ldw * z % 16 == 0 && a.w_stride * z % 16 == 0 &&
                     a.k * z % 16 == 0;
     // Which kernel, by the rows an expert has on average (the host does not know the offsets) and the tiles there can be.
-    // Microseconds of the taken side and of the other, skewed loads, cold memory:
-    //   narrow    798720 rows 48 -> 32 int8            33, tiles 136
-    //   rows      64 over 64 experts, 1024 x 2048      34, 128 x 128 tiles 53;  7 rows 157 x 3840: 8 k groups 8.5, 4 26
-    //             128 over 16, 2048 x 2048             30, 16 rows a workgroup 36;  200 over 8, 300 x 1000: 7.5, 64 x 64 tiles 8.8
-    //             float32 400 over 8, 300 x 2001        23, 64 x 64 tiles 93;  500 of one, 900 x 1024: 22, 64 x 64 24
-    //   64 x 64   1024 over 16, 1024 x 1024            13, 128 x 128 20;  512 over 4, 1024 x 1024: 9.5, rows 20;
-    //             float32 5000 over 5, 1000 x 2000    201, 128 x 128 254
-    //             float32 1000 of one, 800 x 1000      26, rows 37
-    //   128 x 128 8900 over 22, 1424 x 1944           134, 256 x 256 167;  8192 over 64, 2048 x 2048: 176, 256 x 256 216
-    //             short k: 16384 over 8, 1024 x 512     37, 256 x 256 41;  int8 8192 over 16, 2048 x 1024: 37, 256 x 256 42
-    //   256 x 256 16384 over 16, 4096 x 2048          327, 128 x 128 403;  int8 6000 over 8, 2048 x 2048: 40, 128 x 128 49
-    //             4096 of one, 4096 x 4096            119, 128 x 128 165;  16384 over 16, 1024 x 2048: 93, 128 x 128 98
+    // Microseconds of the taken side and of the other: a call of a captured graph of calls, median of 9, inputs cold (copies of the
+    // buffers in turn), skewed loads, rows gathered and scaled, bias and ReLU (lines marked *: the cases of perf/operators.py);
+    // bfloat16 where no type is named:
+    //   narrow    798720 rows 48 -> 32 int8 *          53, tiles 76
+    //   rows      64 over 64 experts, 1024 x 2048 *    39, 128 x 128 tiles 51;  7 rows 157 x 3840: 8 k groups 8.5, 4 11.8
+    //             128 over 16, 2048 x 2048             34, 16 rows a workgroup 37;  200 over 8, 300 x 1000: 9.6, 64 x 64 tiles 12.2
+    //             float32 400 over 8, 300 x 2001       24, 64 x 64 tiles 124;  500 of one, 900 x 1024: 22, 64 x 64 24
+    //   64 x 64   1024 over 16, 1024 x 1024            19, 128 x 128 20;  512 over 4, 1024 x 1024: 12.1, rows 21
+    //             float32 5000 over 5, 1000 x 2000    200, 128 x 128 253
+    //             float32 1000 of one, 800 x 1000      25, rows 36
+    //   128 x 128 8900 over 22, 1424 x 1944           131, 256 x 256 146;  8192 over 64, 2048 x 2048: 167, 256 x 256 186
+    //             short k: 16384 over 8, 1024 x 512     41, 256 x 256 43;  int8 8192 over 16, 2048 x 1024: 47, 256 x 256 48
+    //   256 x 256 16384 over 16, 4096 x 2048 *        308, 128 x 128 378;  int8 6000 over 8, 2048 x 2048: 44, 128 x 128 53
+    //             4096 of one, 4096 x 4096            118, 128 x 128 170;  16384 over 16, 1024 x 2048: 106, 128 x 128 108
+    // Where the rule is not the faster side: 1024 over 64, 1024 x 1024 (16 rows an expert) rows 52, 64 x 64 tiles 42; 4096 over 8,
+    // 2048 x 4096 128 x 128 116, 256 x 256 101.
     const long long groups = a.rows < a.experts ? a.rows : a.experts, avg = a.rows / a.experts;
     const auto tiles = [&](long long tm, long long tn) { return (a.rows / tm + groups) * ((a.n + tn - 1) / tn); };
     if (a.n <= 64 && a.k * z <= 256 && avg >= 512) {
@@ -799,7 +804,7 @@ static hipError_t pick(qcnn_grouped_matmul_t a, hipStream_t s)
         return a.n <= 32 ? run_narrow<T, 2, 4>(a, s) : run_narrow<T, 4, 4>(a, s);
     }
     if (tiles(32, 32) < 128) return run_rows<T, 1, 256, 8, 1, 160>(a, al, s);
-    if (avg <= 24 && a.k * z <= 512) return run_rows<T, 1, 256, 1, 4, 40>(a, al, s);  // nothing to split k for: 61 rows over 82, 2334 x 71 int8: 11 us, split 31
+    if (avg <= 24 && a.k * z <= 512) return run_rows<T, 1, 256, 1, 4, 40>(a, al, s);  // nothing to split k for: 61 rows over 82, 2334 x 71 int8: 14.8 us, split 35
     if (avg <= 4) return run_rows<T, 1, 128, 4, 2, 80>(a, al, s);
     if (tiles(64, 64) < (sizeof(T) == 4 ? 160 : 64)) return run_rows<T, 2, 128, 4, 2, 80>(a, al, s);
     if (avg <= 24) return run_rows<T, 4, 128, 2, 4, 80>(a, al, s);

@@ -8,10 +8,10 @@
 //
 // The waves of a workgroup are KW x NW: NW share out the outputs, 16 NT each, KW the k, in runs of 128, and the KW sums
 // meet in LDS at the end.  Everything goes through LDS, brought there by direct loads R - 1 runs ahead of its use, so that
-// a wave has kilobytes on their way without registers for them.  A wave issues an instruction every seven cycles or so, so
+// a wave has kilobytes on their way without registers for them (R is what LDS holds: 2 to 8; 2 for 5 to 16 rows and many outputs).  A wave issues an instruction every seven cycles or so, so
 // instructions a run and waves on a CU set the pace where the memory does not.  A wave brings its own codes and scales; x is
 // shared by the NW waves of a k group, one barrier a run, none for NW = 1.
-// Measured: 16 half rows, 16384 x 8192, groups of 64 with zeros: 21 us, 3.5 TB/s; one bfloat16 row, 4096 x 4096: 4.6 us.
+// Measured, weights cold: 16 half rows, 16384 x 8192, groups of 64 with zeros: 27.5 us, 2.7 TB/s; one bfloat16 row, 4096 x 4096: 5.8 us.
 // Of 128 k a lane holds 16 bytes of each of its weight rows: lane l, row l & 15, k from (l >> 4) * 32 on.  Instruction j
 // of four wants k = 32 j + (l >> 4) * 8 there, so that its 32 k lie in one group: a 4 x 4 transposition of dwords among
 // the lanes l, l + 16, l + 32, l + 48, four swaps of rows of lanes.
@@ -20,10 +20,12 @@
 // to the fraction by the same multiplication, has both in place, one in each half; and-or cuts them out and puts the
 // exponents in: two operations for two weights, of which the multiplication picks the byte by itself.  The 16 and the
 // zero point leave by the sum of x, a product of the same operand with ones:  sum (16 + q) x - (16 + z) sum x.  (Numbers of
-// 16 to 31 where -8 to 7 are meant cost five times the rounding of a float32 sum; exact codes, -8 to 7 by v_cvt_off_f32_i4 or
+// 16 to 31 where -8 to 7 are meant cost five times the rounding that -8 to 7 have: in the mean 1.0e-7 to 2.5e-7 of the L2 norm
+// of an output's terms at k = 4096, where the library's float32 product has 5.7e-7.  Exact codes, -8 to 7 by v_cvt_off_f32_i4 or
 // by half arithmetic, took 12 to 14 operations for 8 weights in place of 8 and the time was theirs.)
-// float32 x: three bfloat16 parts (8 + 8 + 8 bits, exact), three instructions.  Its results have the bits to show the rounding
-// of larger sums and its time is that of the parts, so its codes are q - 8, and the sum of x comes in only with zero points.
+// float32 x: three bfloat16 parts (8 + 8 + 8 bits; exact down to 2^-109, below that multiples of 2^-133), three instructions.  Its
+// results have the bits to show the rounding of larger sums and its time is that of the parts, so its codes are q - 8, and the
+// sum of x comes in only with zero points.
 #include "block_ops.h"
 
 namespace qcnn {
@@ -267,7 +269,7 @@ __global__ __launch_bounds__(64 * KW *NW) void k_w4(const qcnn_matvec_w4_t a, un
         } else if (cut && i == whole) {  // element by element, zeros behind the end of x
             const int kb = first + i;
             char *at = ring + bring_slot, *mine = at + G::XB + nq * G::WB;
-            // (eight loads on their way at a time: 5 x 1001 x 2047 float32 took 12.5 us with one, 10.7 with eight)
+            // (eight loads on their way at a time: one at a time cost 5 x 1001 x 2047 float32 1.8 us more)
 #pragma unroll 1
             for (int t = 0; t < 2 * NT; ++t) {  // of 8 rows the lane brings byte lane; lane (row + 16 (byte >> 4)) of their tile reads it
                 uint8_t v[8];
@@ -464,18 +466,20 @@ static hipError_t run(const qcnn_matvec_w4_t &a, hipStream_t s)
 
 // Rows of x a workgroup takes and how its waves share out the work.  With few outputs there are few workgroups, each
 // wave is alone with its instructions' latencies, and more waves along k are what helps; with many outputs, sharing x
-// among waves and several workgroups on a CU.  Microseconds at k = 4096, cold memory, group 128, for n = 1024 / 4096 / 8192 /
-// 16384, the taken side of each border first:
-//   bfloat16 rows <= 4     4.6 / 4.9 / 7.2 / 11.0   (KB 80: 4.7 / 5.4 / 7.6 / 12.9;  two tiles a wave 6.1 / 6.3 / 7.4 / 10.8)
-//            rows <= 16    8 x 1 5.5 / 6.4 / 12.0 / 21.9 up to 4096, 4 x 2 7.6 / 8.1 / 9.1 / 14.2 above
-//            64 rows       32 rows 4 x 2 9.5 / 11.0 / 20.4 / 40.1 up to 4096, 4 x 4 12.9 / 14.4 / 15.7 / 31.3 up to 8192 (and up
-//                          to 32 rows), 64 rows 2 x 4 20.5 / 22.4 / 23.0 / 26.8 above
-//   float32  rows <= 4     one tile 7.4 / 8.1 / 13.5 / 22.9 up to 4096, two 8.6 / 9.2 / 10.2 / 16.9 above
-//            rows <= 16    one tile 13.1 / 14.1 / 15.5 / 30.1 up to 8192, two 17.2 / 18.5 / 19.5 / 21.8 above
-//            64 rows       16 rows 4 x 4 20.5 / 24.1 / 44.4 / 96.1 up to 8192 (and up to 32 rows), 32 rows, two tiles 47.2 / 49.4 /
-//                          49.7 / 60.1 above
+// among waves and several workgroups on a CU.  Microseconds at k = 4096, group 128, for n = 1024 / 4096 / 8192 / 16384 (a call of a
+// captured graph of calls, median of 9, weights cold), the taken side of each border first:
+//   bfloat16 rows <= 4     4.7 / 5.8 / 7.6 / 11.5   (KB 80: 4.7 / 6.0 / 8.0 / 13.2;  two tiles a wave 6.1 / 7.0 / 7.5 / 11.2)
+//            rows <= 16    8 x 1 5.4 / 6.9 / 11.8 / 22 up to 4096, 4 x 2 7.5 / 8.3 / 8.8 / 13.9 above
+//            32 rows       4 x 2 9.3 / 10.8 / 11.4 / 21.2 up to 4096, 4 x 4 12.4 / 14.1 / 14.3 / 16.6 above
+//            64 rows       32 rows 4 x 2 9.4 / 11.0 / 20.0 / 38 up to 4096, 4 x 4 12.4 / 13.8 / 15.3 / 28.4 up to 8192, 64 rows 2 x 4
+//                          20.8 / 22.6 / 22.8 / 25.0 above
+//   float32  rows <= 4     one tile 7.4 / 8.0 / 12.0 / 21.0 up to 4096, two 8.8 / 9.4 / 9.9 / 16.3 above
+//            rows <= 16    one tile 12.8 / 14.1 / 14.6 / 27.1 up to 8192, two 17.6 / 19.3 / 19.7 / 21.1 above
+//            64 rows       16 rows 4 x 4 20.2 / 21.2 / 40.2 / 79 up to 8192 (and up to 32 rows), 32 rows, two tiles 45 / 47 / 48 / 49.4
+//                          above
+// (Not the faster side: bfloat16 32 rows at n = 8192 4 x 2 11.4; float32 16 rows at n = 4096 8 x 1 9.8.)
 // Where that leaves fewer than 128 workgroups, sixteen rows and sixteen outputs each with the most waves along k that fit:
-// 9 x 167 x 12134 float32 56 -> 25 us, 22 x 128 x 10048 bfloat16 25 -> 11.
+// 9 x 167 x 12134 float32 46 -> 21 us, 22 x 128 x 10048 bfloat16 22 -> 11.6.
 template <typename T, int FL>
 static hipError_t pick_rows(const qcnn_matvec_w4_t &a, hipStream_t s)
 {

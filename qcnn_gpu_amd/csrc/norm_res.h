@@ -7,8 +7,9 @@
 // input is read once and every output written once, the floor of the operator.  A thread holds CPT chunks of 16 bytes,
 // chunk c of a row belonging to thread c mod LPR, so that neighbouring threads touch neighbouring addresses.
 // Loads and stores take any alignment; only the chunk that the end of a row cuts goes by elements.
-// The memory bounds it: 16384 x 4096 bfloat16 with a gate, 5 arrays: 136 us, 4.9 TB/s; 4096 x 2048 half, eight gathered rows
-// each: 43 us, 4.3 TB/s; one row of 4096: 3.8 us, the latency of one load, two sums and one store.
+// The memory bounds it.  Measured here and below: a call of a captured graph of calls, median of 9, inputs cold: 16384 x 4096 bfloat16 with
+// a gate, 5 arrays: 136 to 139 us, 4.8 to 4.9 TB/s; 4096 x 2048 half, eight gathered rows each: 43 to 47 us, 4.0 to 4.3 TB/s; one row of
+// 4096: 3.7 us, the latency of one load, two sums and one store.
 // Statistics are float32 (the variance as the mean of the squared distances from the mean, from the registers).
 #pragma once
 #include "block_ops.h"
@@ -267,9 +268,9 @@ template <typename T, int LPR, int CPT>
 static hipError_t run(const qcnn_norm_res_t &a, hipStream_t s)
 {
     constexpr int BLOCK = LPR > 256 ? LPR : 256, RPB = BLOCK / LPR;
-    // Outputs from 8 MB on are written past the caches: 2048 x 8192 bf16 36.4 -> 28.8 us, 16384 x 4096 156 -> 152.  A reader right behind
-    // takes as long either way (4096 x 1024 and two readers 18.8 -> 17.8, 16384 x 4096 207 -> 206), but finds smaller ones sooner in
-    // the caches (256 x 4096 and two readers 11.6, 12.0 past them).
+    // Outputs from 8 MB on are written past the caches: 2048 x 8192 bf16 42.8 -> 38.1 us, 16384 x 4096 112.5 -> 109.6
+    // (with a gate 142 -> 138), 4096 x 2048 half of eight parts 47.0 -> 43.4.  With copies of h and n right behind, 16384 x 4096 210 -> 206,
+    // but 4096 x 1024 (16 MB) 19.2 -> 19.6; 256 x 4096 10.5 either way.
     const bool stream = (size_t)a.rows * a.d * sizeof(T) * ((a.h != nullptr) + (a.n != nullptr)) >= (size_t)8 << 20;
     // A launch's threads have to stay below 2^32: more rows take several, that part where a row of gate does, or inside one.
     const long long most = (0xffffffffu / BLOCK) * (long long)RPB, gate_rows = a.gate ? a.gate_rows : 1;
@@ -297,8 +298,8 @@ static hipError_t run(const qcnn_norm_res_t &a, hipStream_t s)
 }
 
 // Threads a row and chunks a thread.  A row of at most 64 chunks fits one wave (no barrier).  With up to 512 rows the time is one
-// row's latency: a chunk a thread (1 x 4096 bf16 5.2 -> 3.9 us, 256 x 8192 10.1 -> 6.7); with more, two and four chunks a thread keep
-// more rows on a CU (16384 x 4096: 156 us, 170 with one; 2048 x 8192: 36.4, 42.6 with one).
+// row's latency: a chunk a thread (1 x 4096 bf16 5.1 -> 3.7 us, 256 x 8192 12.8 -> 7.3); with more, two and four chunks a thread keep
+// more rows on a CU (16384 x 4096: 110 us, 125 with one; 2048 x 8192: 38.1, 42.1 with one).
 template <typename T>
 hipError_t norm_res_of(const qcnn_norm_res_t &a, hipStream_t s)
 {

@@ -272,3 +272,18 @@ def test_grouped_error_of_long_rows(sizes, n, k, kind):
     x, w = (t.to(T[kind]).double().square() for t in (x, w.view(e, n, k)))
     l2 = torch.cat([p @ v.t() for p, v in zip(x.split(sizes), w)]).sqrt().numpy()
     assert rms(y.double().cpu().numpy() - want) <= rms(2 * U * np.sqrt(k / 6) * l2 + U * np.abs(want))
+
+
+def test_w4_float32_rows_of_small_values():
+    """A float32 value goes in as three bfloat16 parts, so as a multiple of 2^-133: full precision from 2^-109 on, below that off by
+    at most 2^-133 of every value times what it is multiplied with."""
+    for shift in (-100, -108, -115, -122, -130):
+        g = torch.Generator().manual_seed(-shift)
+        x = torch.randn(4, 256, generator=g, dtype=torch.float64)
+        x = torch.where(x.abs() < 0.5, x.sign() * 0.5 + x / 2, x) * 2.0 ** shift  # at least 2^(shift - 1)
+        w = torch.randint(0, 256, (48, 128), generator=g, dtype=torch.uint8)
+        scale, zero = (torch.rand(4, 48, generator=g) + 0.5).double(), torch.randint(0, 16, (4, 48), generator=g, dtype=torch.uint8)
+        y, want, bound = w4_run(x, w, scale, zero, None, 64, "f32")
+        q = np.stack((w.numpy() & 15, w.numpy() >> 4), -1).reshape(48, 256).astype(np.float64)
+        size = (scale.float().double().repeat_interleave(64, 0).T.numpy() * (np.abs(q - 8) + np.abs(zero.repeat_interleave(64, 0).T.double().numpy() - 8))).sum(1)
+        close(y, want, bound + (2.0 ** -133 * size[None, :] if shift < -108 else 0), "f32", shift)
