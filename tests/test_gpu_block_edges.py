@@ -287,3 +287,51 @@ def test_w4_float32_rows_of_small_values():
         q = np.stack((w.numpy() & 15, w.numpy() >> 4), -1).reshape(48, 256).astype(np.float64)
         size = (scale.float().double().repeat_interleave(64, 0).T.numpy() * (np.abs(q - 8) + np.abs(zero.repeat_interleave(64, 0).T.double().numpy() - 8))).sum(1)
         close(y, want, bound + (2.0 ** -133 * size[None, :] if shift < -108 else 0), "f32", shift)
+
+
+# ---- the largest values and sizes of single arguments ----------------------------------------------------
+def test_grouped_int8_sums_at_the_end_of_int32():
+    """k = 131071 times 128 * 128 is the largest sum an int32 holds; in the kernels that split k and in those that do not."""
+    k = 131071
+    for sizes, n in (([2], 5), ([130, 120], 300), ([700], 1200)):
+        e, rows = len(sizes), sum(sizes)
+        x, w = torch.full((rows, k), -128, dtype=torch.int8, device="cuda"), torch.full((e, n, k), -128, dtype=torch.int8, device="cuda")
+        w[:, 1] = 127
+        off, y = torch.tensor([0] + sizes).cumsum(0).to(torch.int32).cuda(), torch.zeros(rows, n, device="cuda")
+        call(capi.load().qcnn_op_grouped_matmul, capi.GroupedMatmul(x=ptr(x), y=ptr(y), w=ptr(w), offsets=ptr(off), ldx=k, ldy=n, ldw=k, w_stride=n * k, rows=rows,
+             x_rows=rows, experts=e, n=n, k=k, type=capi.I8, out_type=capi.F32))
+        want = torch.full((n,), float(k * 128 * 128), device="cuda")
+        want[1] = float(-k * 128 * 127)
+        assert torch.equal(y, want.expand(rows, n))
+
+
+@pytest.mark.parametrize("kind", ("f32", "bf16"))
+def test_w4_one_group_longer_than_any_row_and_the_longest_row(kind):
+    for rows, n, k, group in ((2, 20, 200, 1 << 30), (1, 3, 1 << 24, 1 << 24), (6, 2, (1 << 23) + 77, 96)):
+        g = torch.Generator().manual_seed(k)
+        x = torch.randint(-1, 2, (rows, k), generator=g, dtype=torch.int8).to(T[kind]).cuda()
+        w = torch.randint(0, 256, (n, (k + 1) // 2), generator=g, dtype=torch.uint8).cuda()
+        s = torch.ones(-(-k // group), n, device="cuda")
+        y = torch.zeros(rows, n, device="cuda")
+        call(capi.load().qcnn_op_matvec_w4, capi.MatvecW4(x=ptr(x), y=ptr(y), w=ptr(w), scale=ptr(s), ldx=k, ldy=n, ldw=(k + 1) // 2, rows=rows, n=n, k=k, group=group,
+             type=KIND[kind], scale_type=capi.F32, out_type=capi.F32))
+        codes = torch.stack((w & 15, w >> 4), -1).view(n, -1)[:, :k].double() - 8
+        assert torch.equal(y.double(), x.double() @ codes.t())  # whole numbers below 2^24
+
+
+@pytest.mark.parametrize("kind,d,rows", (("f32", 1001, 3000), ("bf16", 4099, 2000), ("f16", 77, 60000)))
+def test_norm_in_place_past_the_caches(kind, d, rows):
+    """Outputs of 8 MB and more are written past the caches, also over the inputs that a thread has just read."""
+    g = torch.Generator("cuda").manual_seed(d)
+    x, y = (torch.randn(rows, d, generator=g, device="cuda").to(T[kind]) for _ in range(2))
+    out = []
+    for over in (False, True):
+        xs, ys = x.clone(), y.clone()
+        h, n = (xs, ys) if over else (torch.empty_like(x), torch.empty_like(x))
+        call(capi.load().qcnn_op_norm_res, capi.NormRes(x=ptr(xs), y=ptr(ys), h=ptr(h), n=ptr(n), ldx=d, ldy=d, ldh=d, ldn=d, rows=rows, y_rows=rows, d=d, parts=1,
+             type=KIND[kind], w_type=capi.F32, post=capi.NORM_RMS, pre=capi.NORM_LAYER, alpha=0.5, beta=1.0, post_eps=1e-6, pre_eps=1e-6))
+        out.append((h, n))
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+    v = y.double()
+    want = x.double() + 0.5 * v / (v.square().mean(1, keepdim=True) + 1e-6).sqrt()
+    assert (out[1][0].double() - want).abs().max() <= 8 * torch.finfo(T[kind]).eps + 1e-5
